@@ -259,6 +259,70 @@ void stochqn_hip_comm_finalize(void);
  * alike.  Median and minimum in microseconds.  0, -1 when no reducer is installed, -1000 on failure. */
 int stochqn_hip_comm_allreduce_probe(int count, int reps, double *median_us, double *min_us);
 
+/* ---- first-order steps over the tensors of a model ------------------------------------------------------
+ * The AdamW step over many tensors at once and the norm of all their gradients: what a model is trained with before, or beside,
+ * the quasi-Newton steps above, which take one flat vector.  Independent of real_t: a tensor is f32, bf16 or f16 in either build.
+ * Everything is device memory of one device; the calls work on the stream they are given (a hipStream_t of that device, NULL = its
+ * NULL stream), in order with it, whichever device is current; they allocate nothing, copy nothing, do not synchronise and may be
+ * captured into a graph.  They have no context, so the built-in profiler does not see them.
+ * A list names tensors: contiguous, aligned to their element size, of any length (0 included: the address is not looked at).  The
+ * state of a parameter of k elements starts at a multiple of 128 elements and takes the next multiple of 128 from k on.
+ * Handles may be used by several threads at once; calls that write the same arrays have to be ordered by their caller, by stream. */
+enum { stochqn_hip_f32 = 0, stochqn_hip_bf16 = 1, stochqn_hip_f16 = 2 };
+typedef struct stochqn_hip_tensors stochqn_hip_tensors;
+typedef struct stochqn_hip_adamw stochqn_hip_adamw;
+
+/* NULL on invalid input (not device memory, another device, past the end of its allocation, misaligned), with the reason on stderr. */
+stochqn_hip_tensors *stochqn_hip_tensors_create(int count, void *const ptr[], const size_t size[], const int type[]);
+/* The same tensors at other addresses.  Graphs captured before keep the old ones.  0 or -1000 (the list is then as before). */
+int stochqn_hip_tensors_rebind(stochqn_hip_tensors *tensors, void *const ptr[]);
+void stochqn_hip_tensors_destroy(stochqn_hip_tensors *tensors);
+/* Elements of the state of a list; offset[i] (nullable): where tensor i's begins. */
+size_t stochqn_hip_tensors_state(const stochqn_hip_tensors *tensors, size_t offset[]);
+
+/* out[0] = |grad_scale| * sqrt(sum of all squares), out[1] = grad_scale * min(1, max_norm / out[0]): what the gradients are to be
+ * multiplied with so that their norm, grad_scale (1 / loss scale) included, is at most max_norm (> 0; infinity: no clipping).  A norm
+ * that is not finite makes out[1] NaN, which the step below takes as "reject".  Sums in f64, in an order that depends on the sizes
+ * alone.  work: stochqn_hip_tensors_norm_work() doubles that nothing else uses until the call's work is done.  With a communicator or
+ * reducer installed the tensors are this rank's share and the sum is over all ranks (one double; every rank makes the call), like
+ * every other sum of the library; work[0] holds it afterwards.  Returns 0 or -1000. */
+size_t stochqn_hip_tensors_norm_work(const stochqn_hip_tensors *tensors);
+int stochqn_hip_tensors_norm(stochqn_hip_tensors *tensors, double grad_scale, double max_norm, float out[], double work[], void *hip_stream);
+
+/* AdamW.  With g = *grad_scale * gradient and t = count[0] + 1, for every element, in f32:
+ *   m <- beta1 m + (1 - beta1) g;  v <- beta2 v + (1 - beta2) g^2
+ *   w <- w (1 - step_size weight_decay) - step_size / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+ * then count[0] <- t.  The arrays are the caller's, zero before the first step:
+ *   state_bits = 32   m, v: f32[state]; m_scale, v_scale: NULL
+ *   state_bits = 8    m: e4m3 (OCP), v: e5m2 (OCP) codes, uint8[state]; m_scale, v_scale: uint8[state / 128], the exponent byte of a power
+ *                     of two (e8m0) that 128 elements share.  A moment is code * scale, rounded stochastically -- to one of its two
+ *                     neighbours, each as often as the mean asks for; rounding to nearest would never move v again, which changes by
+ *                     1 - beta2 a step -- by words that depend on (seed, t, place) alone.  v > 0 is held above zero.  A block in which a
+ *                     moment is not finite reads as NaN from then on.
+ *   master            f32[state] or NULL: weights that the step is taken on where a parameter has 16 bits (the parameter is written, rounded,
+ *                     and not read); unused for f32 parameters
+ *   stochastic        without master: bf16 parameters are rounded stochastically as well (no f16 parameters then)
+ *   decay             one byte per tensor, 0: no weight decay for it; NULL: all decay
+ *   count             two int64: steps taken; zero (arrivals within a step)
+ * m, v, master aligned to 16 bytes.  eps >= 2^-126.  No two arrays that the step writes may overlap, nor a gradient with one.
+ * step:  grads: as many tensors, of the same sizes, f32 / bf16 / f16 each; step_size_dev (nullable): a float on the device in place of
+ * step_size (schedules in a captured graph); grad_scale (nullable = 1): a float on the device, out + 1 of the norm.  Not finite: the step
+ * is rejected, nothing is written and nothing counted -- the guard of take_step, left on the device.  Returns 0 or -1000. */
+typedef struct stochqn_hip_adamw_setup {
+	double beta1, beta2, eps, weight_decay;
+	int state_bits, stochastic;
+	unsigned long long seed;
+	const unsigned char *decay;
+	float *master;
+	void *m, *v;
+	unsigned char *m_scale, *v_scale;
+	long long *count;
+} stochqn_hip_adamw_setup;
+stochqn_hip_adamw *stochqn_hip_adamw_create(stochqn_hip_tensors *params, const stochqn_hip_adamw_setup *setup);
+int stochqn_hip_adamw_step(stochqn_hip_adamw *opt, stochqn_hip_tensors *grads, double step_size, const float *step_size_dev,
+	const float *grad_scale, void *hip_stream);
+void stochqn_hip_adamw_destroy(stochqn_hip_adamw *opt);
+
 /* ---- event counters ---------------------------------------------------------------------------------
  * Process-wide counts since start (or the last reset).  Names:
  *   "steps_three_pass", "steps_sweeps"  take_step calls with pairs in memory, by the

@@ -62,6 +62,7 @@ def lib(use_float=False):
     return _bound[key]
 
 
+from .adamw import AdamW_free, TensorList  # noqa: E402
 from .free import oLBFGS_free, SQN_free, adaQN_free  # noqa: E402
 
-__all__ = ["lib", "cdll", "LIB_PATH", "oLBFGS_free", "SQN_free", "adaQN_free"]
+__all__ = ["lib", "cdll", "LIB_PATH", "oLBFGS_free", "SQN_free", "adaQN_free", "AdamW_free", "TensorList"]

@@ -1,0 +1,261 @@
+"""First-order steps over the tensors of a model: AdamW with its moments in 32 or in 8 bits, and the norm of all gradients.
+
+The object mirrors the free-mode optimisers of `free.py` -- the caller computes gradients, hands them over with `update_gradient` and
+asks for a step with `run_optimizer(step_size)` -- for parameters that are many tensors (f32, bf16, f16) instead of one flat vector.
+The arithmetic is the library's (include/stochqn_hip.h, "first-order steps"); all of it runs on the current torch stream, in order
+with it, without a synchronisation, and may be captured into a graph.
+"""
+import ctypes as C
+import math
+
+BLOCK = 128                     # elements that share a scale; every tensor's state starts at a multiple of it
+
+
+class _Setup(C.Structure):
+    _fields_ = [("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+                ("state_bits", C.c_int), ("stochastic", C.c_int), ("seed", C.c_ulonglong), ("decay", C.c_char_p),
+                ("master", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("m_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("count", C.c_void_p)]
+
+
+_lib = None
+
+
+def _library():
+    global _lib
+    if _lib is None:
+        from . import cdll
+        h = cdll()
+        vp, pp, sz, d, i = C.c_void_p, C.POINTER(C.c_void_p), C.c_size_t, C.c_double, C.c_int
+        for name, result, args in (
+                ("stochqn_hip_tensors_create", vp, [i, pp, C.POINTER(sz), C.POINTER(i)]),
+                ("stochqn_hip_tensors_rebind", i, [vp, pp]),
+                ("stochqn_hip_tensors_destroy", None, [vp]),
+                ("stochqn_hip_tensors_state", sz, [vp, C.POINTER(sz)]),
+                ("stochqn_hip_tensors_norm_work", sz, [vp]),
+                ("stochqn_hip_tensors_norm", i, [vp, d, d, vp, vp, vp]),
+                ("stochqn_hip_adamw_create", vp, [vp, C.POINTER(_Setup)]),
+                ("stochqn_hip_adamw_step", i, [vp, vp, d, vp, vp, vp]),
+                ("stochqn_hip_adamw_destroy", None, [vp])):
+            f = getattr(h, name)
+            f.restype, f.argtypes = result, args
+        _lib = h
+    return _lib
+
+
+def _types():
+    import torch
+    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _scalar(t, device, what):
+    """Address of a device tensor of one float32 (None: none)."""
+    import torch
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
+        raise ValueError("'%s' has to be a float32 tensor of one element on %s." % (what, device))
+    return t.data_ptr()
+
+
+class TensorList:
+    """Tensors of one device (parameters, or their gradients) as the library takes them: contiguous, float32 / bfloat16 / float16 each.
+
+    The list keeps the tensors alive.  `rebind(tensors)` names other ones of the same sizes and types; a graph that was captured before
+    goes on with those it saw."""
+
+    _handle = None
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        types = _types()
+        if not self.tensors:
+            raise ValueError("no tensors.")
+        self.device = getattr(self.tensors[0], "device", None)
+        for t in self.tensors:
+            if getattr(t, "dtype", None) not in types:
+                raise ValueError("tensors have to be float32, bfloat16 or float16.")
+        self._check(self.tensors)
+        n = len(self.tensors)
+        self.sizes = [t.numel() for t in self.tensors]
+        self.dtypes = [t.dtype for t in self.tensors]
+        self._lib = _library()
+        self._at = [t.data_ptr() for t in self.tensors]
+        self._handle = self._lib.stochqn_hip_tensors_create(n, (C.c_void_p * n)(*self._at), (C.c_size_t * n)(*self.sizes),
+                                                            (C.c_int * n)(*[types[d] for d in self.dtypes]))
+        if not self._handle:
+            raise ValueError("the library refused the tensors (its reason is on stderr).")
+        self._work = self._lib.stochqn_hip_tensors_norm_work(self._handle)
+
+    def _check(self, tensors):
+        for t in tensors:
+            if not t.is_cuda or t.device != self.device:
+                raise ValueError("tensors have to be on one GPU.")
+            if not t.is_contiguous():
+                raise ValueError("tensors have to be contiguous.")
+
+    def rebind(self, tensors):
+        """Other tensors of the same sizes and types take the place of the list's (new gradients of the same parameters)."""
+        tensors = list(tensors)
+        if [t.numel() for t in tensors] != self.sizes or [t.dtype for t in tensors] != self.dtypes:
+            raise ValueError("the tensors have other sizes or types than the list's.")
+        self._check(tensors)
+        at = [t.data_ptr() for t in tensors]
+        if at != self._at:
+            if self._lib.stochqn_hip_tensors_rebind(self._handle, (C.c_void_p * len(at))(*at)) != 0:
+                raise ValueError("the library refused the tensors (its reason is on stderr).")
+            self._at = at
+        self.tensors = tensors
+
+    def __len__(self):
+        return len(self.tensors)
+
+    def norm(self, max_norm=None, grad_scale=1.0, out=None):
+        """A float32 tensor of two elements on the device: the norm over all tensors times `grad_scale` (1 / loss scale), and the factor
+        that brings the gradients to a norm of at most `max_norm` -- NaN if the norm is not finite, which makes the step that takes it
+        (`run_optimizer(..., grad_scale=out[1:])`) a rejected one.  With a communicator installed: over all ranks' tensors."""
+        import torch
+        max_norm = math.inf if max_norm is None else float(max_norm)
+        if not max_norm > 0 or not math.isfinite(grad_scale):
+            raise ValueError("'max_norm' has to be positive and 'grad_scale' finite.")
+        if out is None:
+            out = torch.empty(2, dtype=torch.float32, device=self.device)
+        elif out.dtype != torch.float32 or out.shape != (2,) or out.device != self.device or not out.is_contiguous():
+            raise ValueError("'out' has to be a float32 tensor of two elements on %s." % self.device)
+        work = torch.empty(self._work, dtype=torch.float64, device=self.device)      # of this call alone: two streams, or two graphs, share none
+        stream = torch.cuda.current_stream(self.device).cuda_stream
+        if self._lib.stochqn_hip_tensors_norm(self._handle, grad_scale, max_norm, out.data_ptr(), work.data_ptr(), stream) != 0:
+            raise RuntimeError("stochqn_hip_tensors_norm failed (its reason is on stderr).")
+        return out
+
+    def __del__(self):
+        if self._handle:
+            self._lib.stochqn_hip_tensors_destroy(self._handle)
+
+
+class AdamW_free:
+    """AdamW, free mode, over a list of tensors.
+
+    params         tensors (or a TensorList): float32, bfloat16, float16, mixed as they come; updated in place
+    state_bits     32: the moments `m`, `v` are float32; 8: float8_e4m3fn / float8_e5m2 codes over float8_e8m0fnu scales of 128
+                   elements (`m_scale`, `v_scale`), rounded stochastically
+    master         keep float32 weights (`master`) for the 16-bit parameters and take the step on those
+    stochastic     without master: round bfloat16 parameters stochastically (no float16 parameters then)
+    decay          one truth value per tensor: False = no weight decay for it (biases, norms); None: all decay
+    The state is flat tensors of `sum(ceil(n / 128) * 128)` elements; tensor i's begins at `offsets[i]`; `count[0]` is the number of steps.
+    """
+
+    _handle = None
+
+    def __init__(self, params, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, state_bits=32, master=False, stochastic=False,
+                 decay=None, seed=0):
+        import torch
+        assert 0 <= beta1 < 1 and 0 <= beta2 < 1
+        assert 2.0 ** -126 <= eps < 3e38 and math.isfinite(weight_decay)
+        assert state_bits in (8, 32)
+        assert not (master and stochastic)
+        self.params = params if isinstance(params, TensorList) else TensorList(params)
+        self.tensors = list(self.params.tensors)        # what the steps write, whatever the list is rebound to later
+        assert not (stochastic and torch.float16 in self.params.dtypes)
+        assert decay is None or len(decay) == len(self.params)
+        self.beta1, self.beta2, self.eps, self.weight_decay = float(beta1), float(beta2), float(eps), float(weight_decay)
+        self.state_bits, self.stochastic, self.seed = int(state_bits), bool(stochastic), int(seed) % 2 ** 64
+        self.decay = None if decay is None else [bool(d) for d in decay]
+        self._lib = _library()
+        dev = self.params.device
+        offsets = (C.c_size_t * len(self.params))()
+        total = self._lib.stochqn_hip_tensors_state(self.params._handle, offsets)
+        self.offsets = list(offsets)
+        zeros = lambda n, dtype: torch.zeros(n, dtype=dtype, device=dev)
+        if self.state_bits == 32:
+            self.m, self.v = zeros(total, torch.float32), zeros(total, torch.float32)
+            self.m_scale = self.v_scale = None
+        else:
+            byte = lambda n, dtype: zeros(n, torch.uint8).view(dtype)
+            self.m, self.v = byte(total, torch.float8_e4m3fn), byte(total, torch.float8_e5m2)
+            self.m_scale, self.v_scale = byte(total // BLOCK, torch.float8_e8m0fnu), byte(total // BLOCK, torch.float8_e8m0fnu)
+        self.count = zeros(2, torch.int64)
+        self.master = None
+        if master:
+            self.master = zeros(total, torch.float32)
+            for t, at in zip(self.tensors, self.offsets):
+                self.master[at:at + t.numel()].copy_(t.detach().reshape(-1))
+        ptr = lambda t: None if t is None else t.data_ptr()
+        setup = _Setup(self.beta1, self.beta2, self.eps, self.weight_decay, self.state_bits, int(self.stochastic), self.seed,
+                       None if decay is None else bytes(self.decay), ptr(self.master), ptr(self.m), ptr(self.v), ptr(self.m_scale),
+                       ptr(self.v_scale), ptr(self.count))
+        self._handle = self._lib.stochqn_hip_adamw_create(self.params._handle, C.byref(setup))
+        if not self._handle:
+            raise ValueError("the library refused the optimizer (its reason is on stderr).")
+        self.gradient = None
+        self._own_list = False          # `gradient` was made here, so its tensors may be exchanged here
+
+    def update_gradient(self, gradient):
+        """Name the gradients of the coming steps: tensors (or a TensorList) in the order of the parameters.  Nothing is copied: the steps
+        read what the tensors hold by then."""
+        if isinstance(gradient, TensorList):
+            if gradient.sizes != self.params.sizes or gradient.device != self.params.device:
+                raise ValueError("the gradients have other sizes or another device than the parameters.")
+            self.gradient, self._own_list = gradient, False
+            return
+        gradient = list(gradient)
+        if [t.numel() for t in gradient] != self.params.sizes:
+            raise ValueError("the gradients have other sizes than the parameters.")
+        if self._own_list and [t.dtype for t in gradient] == self.gradient.dtypes:
+            self.gradient.rebind(gradient)
+            return
+        new = TensorList(gradient)
+        if new.device != self.params.device:
+            raise ValueError("the gradients are on another device than the parameters.")
+        self.gradient, self._own_list = new, True
+
+    def run_optimizer(self, step_size, grad_scale=None):
+        """One step.  step_size: a number, or a float32 tensor of one element on the device (schedules in a captured graph).  grad_scale: None,
+        or such a tensor that every gradient is multiplied with (`TensorList.norm(...)[1:]`); if it is not finite the step is rejected:
+        no weight, no moment and no count changes."""
+        import torch
+        if self.gradient is None:
+            raise ValueError("no gradient: call update_gradient first.")
+        dev = self.params.device
+        step_dev = None
+        if isinstance(step_size, torch.Tensor):
+            step_dev, step_size = _scalar(step_size, dev, "step_size"), 0.0
+        elif not math.isfinite(step_size):
+            raise ValueError("'step_size' is not finite.")
+        scale = _scalar(grad_scale, dev, "grad_scale")
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        if self._lib.stochqn_hip_adamw_step(self._handle, self.gradient._handle, step_size, step_dev, scale, stream) != 0:
+            raise RuntimeError("stochqn_hip_adamw_step failed (its reason is on stderr).")
+
+    def moments(self, i):
+        """The two moments of tensor i as float32, in its shape (copies for 8-bit moments, views otherwise)."""
+        t, at = self.tensors[i], self.offsets[i]
+        out = []
+        for x, by in ((self.m, self.m_scale), (self.v, self.v_scale)):
+            if by is not None:
+                upto = at + -(-t.numel() // BLOCK) * BLOCK
+                x = (x[at:upto].float().view(-1, BLOCK) * by[at // BLOCK:upto // BLOCK].float()[:, None]).view(-1)
+                out.append(x[:t.numel()].view(t.shape))
+            else:
+                out.append(x[at:at + t.numel()].view(t.shape))
+        return tuple(out)
+
+    def state_dict(self):
+        """The state (references, not copies) and the numbers that the steps were taken with."""
+        names = ("m", "v", "m_scale", "v_scale", "master", "count")
+        state = {k: getattr(self, k) for k in names if getattr(self, k) is not None}
+        return dict(state, beta1=self.beta1, beta2=self.beta2, eps=self.eps, weight_decay=self.weight_decay, state_bits=self.state_bits,
+                    stochastic=self.stochastic, seed=self.seed, decay=self.decay, sizes=list(self.params.sizes))
+
+    def load_state_dict(self, state):
+        """Take over the state of another object over tensors of the same sizes, constructed with the same numbers."""
+        mine = self.state_dict()
+        same = ("beta1", "beta2", "eps", "weight_decay", "state_bits", "stochastic", "seed", "decay", "sizes")
+        if set(state) != set(mine) or any(state[k] != mine[k] for k in same):
+            raise ValueError("the state belongs to an optimizer that was constructed otherwise.")
+        for k in set(mine) - set(same):
+            mine[k].copy_(state[k])
+
+    def __del__(self):
+        if self._handle:
+            self._lib.stochqn_hip_adamw_destroy(self._handle)

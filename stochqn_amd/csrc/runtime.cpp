@@ -1347,6 +1347,17 @@ Reducer current_reducer()
 
 void set_thread_reducer(const Reducer& r) { t_reducer = r; }
 
+bool reduce_in_place(double* buf, int count, hipStream_t st)
+{
+	DevCtx c;
+	c.red = current_reducer();
+	if (c.red.kind == Reducer::NONE) return true;
+	(void) take_hip_failure();
+	(c.red.kind == Reducer::LOOP ? loopback_hook : (c.red.kind == Reducer::CUSTOM ? custom_hook : allreduce_hook))(&c, buf, count, st);
+	const bool failed = take_hip_failure();
+	return !c.fault && !failed;
+}
+
 int comm_nranks()
 {
 	const Reducer r = current_reducer();

@@ -306,6 +306,7 @@ struct ApiRange {
 int comm_nranks();
 void comm_attach(DevCtx* c);                           // install the all-reduce hook, compute n_global
 Reducer current_reducer();                             // the calling thread's binding, else the process-wide communicator
+bool reduce_in_place(double* buf, int count, hipStream_t st);   // sum over the ranks of the calling thread's reducer, on the caller's stream (calls without a context)
 void set_thread_reducer(const Reducer& r);             // contexts created by this thread from now on reduce through `r`
 bool comm_init_all(int ndev, const int* devices, void** comms_out);   // ncclCommInitAll (one process, ndev devices)
 void comm_destroy(void* comm);

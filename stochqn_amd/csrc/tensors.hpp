@@ -1,0 +1,68 @@
+// tensors.hpp -- first-order steps over the tensors of a model: what the host side (tensors.cpp) hands to the kernels (tensors.hip).
+// Everything here takes DEVICE pointers and enqueues work on a stream; nothing synchronises, allocates or copies, so that a call
+// can be captured into a graph.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <cstddef>
+#include <cstdint>
+
+namespace sqn {
+
+constexpr int kStateBlock = 128;     // elements that share the scale of an 8-bit moment; every tensor's state starts at a multiple of it
+constexpr int kTile = 2048;          // elements a workgroup of 256 threads takes at a time, eight per lane
+constexpr int kEntries = 112;        // tensors per launch: the table travels in the kernel's arguments (32 B each, 4 KB in all)
+
+enum TensorType { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
+inline size_t type_size(int t) { return t == T_F32 ? 4 : 2; }
+
+// One tensor as a kernel sees it.  `info`: elements (56 bits), the parameter's type (2 bits), the gradient's (2), "no weight decay" (1).
+struct TensorEntry {
+	void* param;
+	const void* grad;
+	uint64_t info;
+	uint32_t tile0;              // first tile of this launch that is the tensor's
+	uint32_t block0;             // first block of kStateBlock elements of its state, counted from AdamwArgs::block_base
+};
+constexpr uint64_t kCountMask = (1ull << 56) - 1;
+inline uint64_t entry_info(size_t count, int ptype, int gtype, bool no_decay)
+{
+	return (uint64_t) count | (uint64_t) ptype << 56 | (uint64_t) gtype << 58 | (uint64_t) no_decay << 60;
+}
+
+struct AdamwArgs {
+	TensorEntry entry[kEntries];
+	int entries;                 // of the table that are in use
+	uint32_t tiles;
+	uint64_t block_base;
+	float* master;               // f32 weights of the 16-bit tensors, or NULL
+	void *m, *v;                 // f32[state] or codes [state]
+	uint8_t *m_scale, *v_scale;  // [state / kStateBlock], 8-bit moments only
+	long long* count;            // [0] steps taken, [1] workgroups that have arrived (zero between steps)
+	const float* grad_scale;     // what every gradient is multiplied with; NULL = 1
+	const float* step_size_dev;  // NULL: step_size
+	double step_size, beta1, beta2, weight_decay;
+	float eps;
+	uint64_t seed;
+	int last;                    // the launch that counts the step
+	int stochastic;              // bf16 parameters without f32 weights beside them are rounded stochastically
+};
+static_assert(sizeof(AdamwArgs) <= 4096, "kernel arguments");
+
+struct NormArgs {
+	TensorEntry entry[kEntries]; // param unused
+	int entries;
+	uint32_t tiles;
+	double* part;                // one partial sum of squares per workgroup of this launch
+	double grad_scale, max_norm;
+	float* out;                  // not NULL: this workgroup, the only one, finishes
+};
+static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
+
+void launch_adamw(hipStream_t st, int bits, int grid, const AdamwArgs& a);
+void launch_norm(hipStream_t st, int grid, const NormArgs& a);
+// part[0] <- the sum of part[1 .. count] (in a fixed order); with `out` also the verdict
+void launch_norm_sum(hipStream_t st, double* part, int count, double grad_scale, double max_norm, float* out);
+// the verdict of a sum of squares that is final: out[0] the norm, out[1] the coefficient
+void launch_norm_verdict(hipStream_t st, const double* sum, double grad_scale, double max_norm, float* out);
+
+}  // namespace sqn
