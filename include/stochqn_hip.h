@@ -304,6 +304,7 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors *tensors, double grad_scale, do
  *   stochastic        without master: bf16 parameters are rounded stochastically as well (no f16 parameters then)
  *   decay             one byte per tensor, 0: no weight decay for it; NULL: all decay
  *   count             two int64: steps taken; zero (arrivals within a step)
+ *   work              64 bytes, aligned to 8, that the steps of this optimizer use between their kernels
  * m, v, master aligned to 16 bytes.  eps >= 2^-126.  No two arrays that the step writes may overlap, nor a gradient with one.
  * step:  grads: as many tensors, of the same sizes, f32 / bf16 / f16 each; step_size_dev (nullable): a float on the device in place of
  * step_size (schedules in a captured graph); grad_scale (nullable = 1): a float on the device, out + 1 of the norm.  Not finite: the step
@@ -317,6 +318,7 @@ typedef struct stochqn_hip_adamw_setup {
 	void *m, *v;
 	unsigned char *m_scale, *v_scale;
 	long long *count;
+	void *work;
 } stochqn_hip_adamw_setup;
 stochqn_hip_adamw *stochqn_hip_adamw_create(stochqn_hip_tensors *params, const stochqn_hip_adamw_setup *setup);
 int stochqn_hip_adamw_step(stochqn_hip_adamw *opt, stochqn_hip_tensors *grads, double step_size, const float *step_size_dev,

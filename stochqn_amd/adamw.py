@@ -15,7 +15,7 @@ class _Setup(C.Structure):
     _fields_ = [("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
                 ("state_bits", C.c_int), ("stochastic", C.c_int), ("seed", C.c_ulonglong), ("decay", C.c_char_p),
                 ("master", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("m_scale", C.c_void_p), ("v_scale", C.c_void_p),
-                ("count", C.c_void_p)]
+                ("count", C.c_void_p), ("work", C.c_void_p)]
 
 
 _lib = None
@@ -174,7 +174,7 @@ class AdamW_free:
             byte = lambda n, dtype: zeros(n, torch.uint8).view(dtype)
             self.m, self.v = byte(total, torch.float8_e4m3fn), byte(total, torch.float8_e5m2)
             self.m_scale, self.v_scale = byte(total // BLOCK, torch.float8_e8m0fnu), byte(total // BLOCK, torch.float8_e8m0fnu)
-        self.count = zeros(2, torch.int64)
+        self.count, self._work = zeros(2, torch.int64), zeros(8, torch.int64)
         self.master = None
         if master:
             self.master = zeros(total, torch.float32)
@@ -183,7 +183,7 @@ class AdamW_free:
         ptr = lambda t: None if t is None else t.data_ptr()
         setup = _Setup(self.beta1, self.beta2, self.eps, self.weight_decay, self.state_bits, int(self.stochastic), self.seed,
                        None if decay is None else bytes(self.decay), ptr(self.master), ptr(self.m), ptr(self.v), ptr(self.m_scale),
-                       ptr(self.v_scale), ptr(self.count))
+                       ptr(self.v_scale), ptr(self.count), ptr(self._work))
         self._handle = self._lib.stochqn_hip_adamw_create(self.params._handle, C.byref(setup))
         if not self._handle:
             raise ValueError("the library refused the optimizer (its reason is on stderr).")

@@ -18,6 +18,13 @@ using namespace sqn;
 
 namespace {
 
+// Most workgroups per compute unit (measured at 1.28e9 elements): 32-bit moments 4, 8 and 16 alike; 8-bit moments 2.53 ms with 8, 2.46 with 16,
+// 2.41 with 32; the norm 466 us with 4, 380 with 8, 384 with 16.
+constexpr int kPerUnit32 = 8, kPerUnit8 = 32, kPerUnitNorm = 8;
+// Up to this many small tiles a step is one launch whose workgroups form its numbers themselves and count it by arrivals, 6.5 ns each;
+// beyond, a kernel in front does (3.5 us in a stream of steps): 7.6 against 11.2 us a step of 57 tiles.
+constexpr uint64_t kAloneTiles = 256;
+
 struct Range { const char* at; size_t bytes; };                              // of device memory
 bool before(const Range& a, const Range& b) { return a.at < b.at; }
 
@@ -60,6 +67,16 @@ void check_memory(const void* p, size_t bytes, int& device, const char* what)
 void check_aligned(const void* p, size_t to, const char* what)
 {
 	if (reinterpret_cast<uintptr_t>(p) % to) refuse(std::string(what) + " is not aligned to " + std::to_string(to) + " bytes");
+}
+
+uint64_t tiles_of(size_t n, int tile) { return (n + tile - 1) / tile; }
+
+// Large tiles keep more loads of a lane in flight; a list that has fewer of them than two for each compute unit is cut into small ones.
+LaunchShape shape_of(const std::vector<Item>& items, int units, int large, int per_unit)
+{
+	uint64_t tiles = 0;
+	for (const Item& it : items) tiles += tiles_of(it.n, large);
+	return {tiles < 2 * (uint64_t) units ? kTileSmall : large, units * per_unit};
 }
 
 size_t blocks_of(size_t n) { return (n + kStateBlock - 1) / kStateBlock; }
@@ -112,9 +129,9 @@ struct stochqn_hip_tensors {
 	std::mutex mu;                     // rebind against the calls that read the addresses
 	std::vector<Item> items;
 	int device = -1;
+	LaunchShape norm{};                // how the norm cuts the list up
 	int units = 0;                     // compute units
 	unsigned long long version = 0;    // another one for every set of addresses
-	size_t biggest_grid() const { return (size_t) units * 4; }
 };
 
 struct stochqn_hip_adamw {
@@ -124,7 +141,8 @@ struct stochqn_hip_adamw {
 	std::vector<size_t> block;         // first block of each tensor's state
 	std::vector<Range> written;        // sorted
 	stochqn_hip_adamw_setup s;
-	int device = -1, units = 0;
+	int device = -1;
+	LaunchShape shape{};
 	unsigned long long checked = 0;    // version of the gradients that have been held against `written`
 };
 
@@ -145,15 +163,15 @@ void set_items(std::vector<Item>& items, int& device, void* const ptr[])
 
 // The tables of a list, one launch after the other: fill(i, entry) for every tensor with elements, fire(base block, entries, tiles) for every
 // table that is full or the last.
-template <class Fill, class Fire> void for_launches(const std::vector<Item>& items, TensorEntry* entry, Fill&& fill, Fire&& fire)
+template <class Fill, class Fire> void for_launches(const std::vector<Item>& items, int tile, TensorEntry* entry, Fill&& fill, Fire&& fire)
 {
 	int used = 0;
 	uint64_t tiles = 0;
 	for (size_t i = 0; i < items.size(); i++) {
 		if (!items[i].n) continue;
-		const uint64_t mine = (items[i].n + kTile - 1) / kTile;
+		const uint64_t mine = tiles_of(items[i].n, tile);
 		if (used == kEntries || (used && tiles + mine > 0x7fffffffu)) {
-			fire(used, (uint32_t) tiles, false);
+			fire(used, (uint32_t) tiles);
 			used = 0;
 			tiles = 0;
 		}
@@ -162,7 +180,7 @@ template <class Fill, class Fire> void for_launches(const std::vector<Item>& ite
 		used++;
 		tiles += mine;
 	}
-	fire(used, (uint32_t) tiles, true);
+	fire(used, (uint32_t) tiles);
 }
 
 }  // namespace
@@ -183,6 +201,7 @@ stochqn_hip_tensors* stochqn_hip_tensors_create(int count, void* const ptr[], co
 		set_items(t->items, t->device, ptr);
 		if (t->device < 0 && hipGetDevice(&t->device) != hipSuccess) refuse("no current device");
 		t->units = units_of(t->device);
+		t->norm = shape_of(t->items, t->units, kTile8, kPerUnitNorm);
 		t->version = ++g_versions;
 		return t.release();
 	});
@@ -218,7 +237,7 @@ size_t stochqn_hip_tensors_norm_work(const stochqn_hip_tensors* t)
 	if (!t) return 0;
 	size_t parts = 0;
 	TensorEntry table[kEntries];
-	for_launches(t->items, table, [](size_t, int) {}, [&](int, uint32_t tiles, bool) { parts += std::min<size_t>(tiles, t->biggest_grid()); });
+	for_launches(t->items, t->norm.tile, table, [](size_t, int) {}, [&](int, uint32_t tiles) { parts += std::min<size_t>(tiles, t->norm.grid); });
 	return 1 + parts;
 }
 
@@ -240,24 +259,23 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors* t, double grad_scale, double m
 		NormArgs a{};
 		a.grad_scale = grad_scale;
 		a.max_norm = max_norm;
-		int parts = 0;
+		int parts = 0, launches = 0;
 		bool done = false;
-		for_launches(t->items, a.entry,
+		for_launches(t->items, t->norm.tile, a.entry,
 			[&](size_t i, int k) {
 				a.entry[k].grad = t->items[i].p;
 				a.entry[k].info = entry_info(t->items[i].n, 0, t->items[i].type, false);
 			},
-			[&](int used, uint32_t tiles, bool last) {
-				if (!used && parts) return;
-				const int grid = (int) std::min<size_t>(std::max<uint32_t>(tiles, 1), t->biggest_grid());
+			[&](int used, uint32_t tiles) {
 				a.entries = used;
 				a.tiles = tiles;
 				a.part = work + 1 + parts;
-				done = last && !parts && grid == 1 && !reduced;        // one workgroup sees everything: it finishes
+				done = tiles <= 1 && !launches && !reduced;             // one workgroup sees everything: it finishes
 				a.out = done ? out : nullptr;
-				if (!used && !done) return;                             // nothing at all, but for a reducer: the sum of no parts
-				launch_norm(st, grid, a);
+				const int grid = (int) std::min<size_t>(done ? 1 : tiles, t->norm.grid);
+				if (grid) launch_norm(st, t->norm.tile, grid, a);
 				parts += grid;
+				launches++;
 			});
 		if (!done) launch_norm_sum(st, work, parts, grad_scale, max_norm, reduced ? nullptr : out);
 		if (reduced) {
@@ -283,7 +301,7 @@ stochqn_hip_adamw* stochqn_hip_adamw_create(stochqn_hip_tensors* params, const s
 		std::lock_guard<std::mutex> lk(params->mu);
 		o->items = params->items;
 		o->device = params->device;
-		o->units = params->units;
+		o->shape = s.state_bits == 8 ? shape_of(o->items, params->units, kTile8, kPerUnit8) : shape_of(o->items, params->units, kTile32, kPerUnit32);
 		o->s = s;
 		size_t blocks = 0;
 		for (size_t i = 0; i < o->items.size(); i++) {
@@ -295,7 +313,7 @@ stochqn_hip_adamw* stochqn_hip_adamw_create(stochqn_hip_tensors* params, const s
 			if (it.n) o->written.push_back({static_cast<char*>(it.p), it.n * type_size(it.type)});
 		}
 		o->s.decay = nullptr;
-		if (!s.count || (blocks && (!s.m || !s.v || (s.state_bits == 8 && (!s.m_scale || !s.v_scale))))) refuse("an array of the state is NULL");
+		if (!s.count || !s.work || (blocks && (!s.m || !s.v || (s.state_bits == 8 && (!s.m_scale || !s.v_scale))))) refuse("an array of the state is NULL");
 		const size_t state = blocks * kStateBlock, moment = state * (s.state_bits / 8);
 		const auto array = [&](const void* p, size_t bytes, size_t to, const char* what) {
 			if (!p || !bytes) return;
@@ -309,6 +327,7 @@ stochqn_hip_adamw* stochqn_hip_adamw_create(stochqn_hip_tensors* params, const s
 		array(s.v_scale, s.state_bits == 8 ? blocks : 0, 1, "v_scale");
 		array(s.master, state * sizeof(float), 16, "master");
 		array(s.count, 2 * sizeof(long long), 8, "count");
+		array(s.work, kStepBytes, 8, "work");
 		std::sort(o->written.begin(), o->written.end(), before);
 		for (size_t i = 1; i < o->written.size(); i++)
 			if (o->written[i - 1].at + o->written[i - 1].bytes > o->written[i].at) refuse("two arrays that the step writes overlap");
@@ -362,7 +381,13 @@ int stochqn_hip_adamw_step(stochqn_hip_adamw* o, stochqn_hip_tensors* grads, dou
 		a.eps = (float) s.eps;
 		a.seed = s.seed;
 		a.stochastic = s.stochastic;
-		for_launches(o->items, a.entry,
+		// few workgroups, one launch: they form the step's numbers themselves; else a kernel in front does
+		uint64_t all = 0;
+		for (const Item& it : o->items) all += tiles_of(it.n, o->shape.tile);
+		const bool alone = o->items.size() <= (size_t) kEntries && all <= kAloneTiles && o->shape.tile == kTileSmall;
+		a.step = alone ? nullptr : static_cast<Step*>(s.work);
+		if (!alone) launch_adamw_begin(st, a);
+		for_launches(o->items, o->shape.tile, a.entry,
 			[&](size_t i, int k) {
 				TensorEntry& e = a.entry[k];
 				if (!k) a.block_base = o->block[i];
@@ -371,11 +396,11 @@ int stochqn_hip_adamw_step(stochqn_hip_adamw* o, stochqn_hip_tensors* grads, dou
 				e.info = entry_info(g[i].n, o->items[i].type, g[i].type, o->no_decay[i]);
 				e.block0 = (uint32_t) (o->block[i] - a.block_base);
 			},
-			[&](int used, uint32_t tiles, bool last) {
+			[&](int used, uint32_t tiles) {
 				a.entries = used;
 				a.tiles = tiles;
-				a.last = last;
-				launch_adamw(st, s.state_bits, (int) std::min<size_t>(std::max<uint32_t>(tiles, 1), (size_t) o->units * 8), a);
+				const int grid = (int) std::min<size_t>(alone ? std::max<uint32_t>(tiles, 1) : tiles, o->shape.grid);
+				if (grid) launch_adamw(st, s.state_bits, o->shape.tile, grid, a);
 			});
 		return launched();
 	});

@@ -11,17 +11,45 @@
 namespace sqn {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));        // parameters and gradients: aligned to their elements only
-typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
 constexpr int kThreads = 256;
-constexpr int kLane = 8;                                                     // elements per lane and tile
-static_assert(kTile == kThreads * kLane, "a tile is eight elements per lane");
+
+// Tensors are aligned to their elements only, the arrays of the state to 16 bytes; global memory takes wide accesses at any address.
+template <int BYTES, int ALIGN> struct Wide;
+#define TS_WIDE(bytes, align) \
+	template <> struct Wide<bytes, align> { typedef uint32_t type __attribute__((ext_vector_type(bytes / 4), aligned(align))); };
+TS_WIDE(16, 16) TS_WIDE(16, 4) TS_WIDE(16, 2) TS_WIDE(8, 8) TS_WIDE(8, 2)
+#undef TS_WIDE
+
+// BYTES bytes (8, 16, 32) from / to global memory
+template <int BYTES, int ALIGN> __device__ inline void fetch(const void* p, uint32_t (&x)[BYTES / 4])
+{
+	constexpr int W = BYTES < 16 ? BYTES : 16;
+	typedef typename Wide<W, ALIGN>::type T;
+#pragma unroll
+	for (int k = 0; k < BYTES / W; k++) {
+		const T t = __builtin_nontemporal_load(static_cast<const T*>(p) + k);
+#pragma unroll
+		for (int j = 0; j < W / 4; j++) x[k * W / 4 + j] = t[j];
+	}
+}
+template <int BYTES, int ALIGN> __device__ inline void put(void* p, const uint32_t (&x)[BYTES / 4])
+{
+	constexpr int W = BYTES < 16 ? BYTES : 16;
+	typedef typename Wide<W, ALIGN>::type T;
+#pragma unroll
+	for (int k = 0; k < BYTES / W; k++) {
+		T t;
+#pragma unroll
+		for (int j = 0; j < W / 4; j++) t[j] = x[k * W / 4 + j];
+		__builtin_nontemporal_store(t, static_cast<T*>(p) + k);
+	}
+}
 
 __device__ inline float bits_float(uint32_t b) { return __builtin_bit_cast(float, b); }
 __device__ inline uint32_t float_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
+
+// V elements of a tensor as they lie in memory: f32 one to a word, 16 bits two to a word (in the first half of the words)
+template <int V> struct Raw { uint32_t w[V]; };
 
 __device__ inline float widen16(uint32_t h, int type)
 {
@@ -32,63 +60,86 @@ __device__ inline uint32_t narrow16(float f, int type)
 	return type == T_BF16 ? (uint32_t) __builtin_bit_cast(uint16_t, (__bf16) f) : (uint32_t) __builtin_bit_cast(uint16_t, (_Float16) f);
 }
 
-// elements i .. i+7 of a tensor of n; what lies behind its end reads as zero
-__device__ inline void load8(const void* base, uint64_t i, uint64_t n, int type, float (&x)[kLane])
+// elements i .. i+V-1 of a tensor of n; what lies behind its end reads as zero
+template <int V> __device__ inline void load(const void* base, uint64_t i, uint64_t n, int type, Raw<V>& x)
 {
-	if (i + kLane <= n) {
-		if (type == T_F32) {
-			const f32x4u* p = reinterpret_cast<const f32x4u*>(static_cast<const float*>(base) + i);
-			const f32x4u a = p[0], b = p[1];
+	if (i + V <= n) {
+		if (type == T_F32) fetch<V * 4, 4>(static_cast<const float*>(base) + i, x.w);
+		else {
+			uint32_t h[V / 2];
+			fetch<V * 2, 2>(static_cast<const uint16_t*>(base) + i, h);
 #pragma unroll
-			for (int j = 0; j < 4; j++) { x[j] = a[j]; x[4 + j] = b[j]; }
-		} else {
-			const u32x4u a = *reinterpret_cast<const u32x4u*>(static_cast<const uint16_t*>(base) + i);
-#pragma unroll
-			for (int j = 0; j < 4; j++) { x[2 * j] = widen16(a[j] & 0xffff, type); x[2 * j + 1] = widen16(a[j] >> 16, type); }
+			for (int j = 0; j < V / 2; j++) x.w[j] = h[j];
 		}
 	} else {
 #pragma unroll
-		for (int j = 0; j < kLane; j++) {
-			x[j] = 0;
-			if (i + j < n) x[j] = type == T_F32 ? static_cast<const float*>(base)[i + j] : widen16(static_cast<const uint16_t*>(base)[i + j], type);
-		}
+		for (int j = 0; j < V; j++) x.w[j] = 0;
+#pragma unroll
+		for (int j = 0; j < V; j++)
+			if (i + j < n) {
+				if (type == T_F32) x.w[j] = static_cast<const uint32_t*>(base)[i + j];
+				else x.w[j / 2] |= (uint32_t) static_cast<const uint16_t*>(base)[i + j] << 16 * (j & 1);
+			}
 	}
 }
-
-__device__ inline void store8(float* base, uint64_t i, uint64_t n, const float (&x)[kLane])
+template <int V> __device__ inline void widen(const Raw<V>& r, int type, float (&x)[V])
 {
-	if (i + kLane <= n) {
-		f32x4u* p = reinterpret_cast<f32x4u*>(base + i);
-		p[0] = f32x4u{x[0], x[1], x[2], x[3]};
-		p[1] = f32x4u{x[4], x[5], x[6], x[7]};
+	if (type == T_F32) {
+#pragma unroll
+		for (int j = 0; j < V; j++) x[j] = bits_float(r.w[j]);
+	} else if (type == T_BF16) {
+#pragma unroll
+		for (int j = 0; j < V; j += 2) { x[j] = bits_float(r.w[j / 2] << 16); x[j + 1] = bits_float(r.w[j / 2] & 0xffff0000u); }
 	} else {
 #pragma unroll
-		for (int j = 0; j < kLane; j++)
+		for (int j = 0; j < V; j += 2) { x[j] = widen16(r.w[j / 2] & 0xffff, T_F16); x[j + 1] = widen16(r.w[j / 2] >> 16, T_F16); }
+	}
+}
+template <int V> __device__ inline void store32(float* base, uint64_t i, uint64_t n, const float (&x)[V])
+{
+	if (i + V <= n) {
+		uint32_t w[V];
+#pragma unroll
+		for (int j = 0; j < V; j++) w[j] = float_bits(x[j]);
+		put<V * 4, 4>(base + i, w);
+	} else {
+#pragma unroll
+		for (int j = 0; j < V; j++)
 			if (i + j < n) base[i + j] = x[j];
 	}
 }
-
-__device__ inline void store8(uint16_t* base, uint64_t i, uint64_t n, const uint32_t (&h)[kLane])
+template <int V> __device__ inline void store16(uint16_t* base, uint64_t i, uint64_t n, const uint32_t (&h)[V / 2])
 {
-	if (i + kLane <= n) {
-		*reinterpret_cast<u32x4u*>(base + i) = u32x4u{h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16};
-	} else {
+	if (i + V <= n) put<V * 2, 2>(base + i, h);
+	else {
 #pragma unroll
-		for (int j = 0; j < kLane; j++)
-			if (i + j < n) base[i + j] = (uint16_t) h[j];
+		for (int j = 0; j < V; j++)
+			if (i + j < n) base[i + j] = (uint16_t) (h[j / 2] >> 16 * (j & 1));
 	}
 }
 
-// the entry of the launch's table that tile `tile` belongs to (uniform over the workgroup)
-template <class Args> __device__ inline int entry_of(const Args& a, uint32_t tile)
-{
-	int lo = 0, hi = a.entries;
-	while (hi - lo > 1) {
-		const int mid = (lo + hi) >> 1;
-		if (a.entry[mid].tile0 <= tile) lo = mid; else hi = mid;
+// the tensor that a workgroup is at: found by bisection once, then followed (its tiles come in rising order)
+template <class Args> struct Cursor {
+	const Args& a;
+	int k;
+	uint32_t next;
+	__device__ Cursor(const Args& args, uint32_t tile) : a(args)
+	{
+		int lo = 0, hi = a.entries;
+		while (hi - lo > 1) {
+			const int mid = (lo + hi) >> 1;
+			if (a.entry[mid].tile0 <= tile) lo = mid; else hi = mid;
+		}
+		k = lo;
+		next = end();
 	}
-	return lo;
-}
+	__device__ uint32_t end() const { return k + 1 < a.entries ? a.entry[k + 1].tile0 : 0xffffffffu; }
+	__device__ const TensorEntry& at(uint32_t tile)
+	{
+		while (tile >= next) { k++; next = end(); }
+		return a.entry[k];
+	}
+};
 
 // ---- stochastic rounding ---------------------------------------------------------------------------------------------------------
 // The moments are running averages: at b2 = 0.999 a step moves v by about a thousandth, while half a step of e5m2 is an eighth -- with
@@ -107,14 +158,13 @@ __device__ inline uint64_t finalise(uint64_t z)
 }
 
 // ---- what is the same for every element of a step ---------------------------------------------------------------------------------
-struct Step {
-	float scale, b1, b2, a1, a2, decay, rate, root, eps;
-	uint64_t key;
-	bool stochastic;
-};
-
 __device__ inline Step step_of(const AdamwArgs& a, long long t)
 {
+	Step s{};
+	// a scale that is not finite: the step is rejected as a whole, nothing changes and nothing is counted
+	s.scale = a.grad_scale ? *a.grad_scale : 1.0f;
+	s.go = fabsf(s.scale) <= 3.402823466e38f;
+	if (!s.go) return s;
 	double p1 = 1, p2 = 1, q1 = a.beta1, q2 = a.beta2;       // b^t by squaring, in f64: 1 - b2^t loses ten bits at t = 1
 	for (unsigned long long k = (unsigned long long) t; k; k >>= 1) {
 		if (k & 1) { p1 *= q1; p2 *= q2; }
@@ -122,7 +172,6 @@ __device__ inline Step step_of(const AdamwArgs& a, long long t)
 		q2 *= q2;
 	}
 	const double lr = a.step_size_dev ? (double) *a.step_size_dev : a.step_size;
-	Step s;
 	s.b1 = (float) a.beta1;
 	s.b2 = (float) a.beta2;
 	s.a1 = (float) (1 - a.beta1);
@@ -133,50 +182,58 @@ __device__ inline Step step_of(const AdamwArgs& a, long long t)
 	s.eps = a.eps;
 	s.key = finalise(a.seed ^ (uint64_t) t * kStepKey);
 	s.stochastic = a.stochastic != 0;
+	s.careful = s.root * 0x1p-63f > s.eps * 0x1p-25f;
 	return s;
 }
 
-// moments and weight of one element
+// Moments and weight of one element.  The hardware's root and reciprocal are within an ulp (1.6 and 1.5 times 2^-24, measured over all
+// exponents), far below the weight's own rounding, and a quarter of the instructions of the exact ones.  The root takes subnormals for
+// zero: their true roots are below 2^-63, nothing beside eps unless eps is tiny (`careful`).
 __device__ inline void update(const Step& s, float decay, float g, float& m, float& v, float& w)
 {
 	m = m * s.b1 + g * s.a1;
 	v = v * s.b2 + (g * g) * s.a2;
-	w = fmaf(-s.rate, m / fmaf(sqrtf(v), s.root, s.eps), w * decay);
+	float q = __builtin_amdgcn_sqrtf(v);
+	if (s.careful && v < 0x1p-64f) q = __builtin_amdgcn_sqrtf(v * 0x1p64f) * 0x1p-32f;
+	w = fmaf(-s.rate, m * __builtin_amdgcn_rcpf(fmaf(q, s.root, s.eps)), w * decay);
 }
 
 // the new weights go out: f32 as they are, 16 bits rounded (to nearest, or stochastically by the low half of the first word: bf16 is
 // the upper half of f32, so the word's 16 bits are added to the lower half and cut off with it)
-__device__ inline void put_weights(const AdamwArgs& a, const Step& s, void* param, uint64_t i, uint64_t n, int ptype, float* master, float (&w)[kLane], uint32_t word)
+template <int V> __device__ inline void put_weights(const Step& s, void* param, uint64_t i, uint64_t n, int ptype, float* master, const float (&w)[V], uint32_t word)
 {
-	if (ptype == T_F32) { store8(static_cast<float*>(param), i, n, w); return; }
-	uint32_t h[kLane];
-	if (master) store8(master, i, n, w);
-	if (!master && s.stochastic) {
+	if (ptype == T_F32) { store32<V>(static_cast<float*>(param), i, n, w); return; }
+	uint32_t h[V / 2];
+	if (master) store32<V>(master, i, n, w);
+	if (ptype == T_F16) {
 #pragma unroll
-		for (int j = 0; j < kLane; j++) {
-			const uint32_t b = float_bits(w[j]);
-			h[j] = ((b & 0x7f800000u) == 0x7f800000u ? (b | (b << 16 ? 0x400000u : 0)) : b + ((word + j * kLaneStep) & 0xffff)) >> 16;
-		}
+		for (int j = 0; j < V; j += 2) h[j / 2] = narrow16(w[j], T_F16) | narrow16(w[j + 1], T_F16) << 16;
+	} else if (s.stochastic) {
+		uint32_t b[V];
+#pragma unroll
+		for (int j = 0; j < V; j++) b[j] = float_bits(w[j]) + (__builtin_isfinite(w[j]) ? (word + j * kLaneStep) & 0xffff : 0u);
+#pragma unroll
+		for (int j = 0; j < V; j += 2) h[j / 2] = __builtin_amdgcn_perm(b[j + 1], b[j], 0x07060302u);
 	} else {
 #pragma unroll
-		for (int j = 0; j < kLane; j++) h[j] = narrow16(w[j], ptype);
+		for (int j = 0; j < V; j += 2) h[j / 2] = narrow16(w[j], T_BF16) | narrow16(w[j + 1], T_BF16) << 16;
 	}
-	store8(static_cast<uint16_t*>(param), i, n, h);
+	store16<V>(static_cast<uint16_t*>(param), i, n, h);
 }
 
 // ---- moments in 8 bits -------------------------------------------------------------------------------------------------------------
 // A block of 128 elements shares a scale 2^k (a byte, the exponent's 8 bits): the largest |m| lies at 2^7 .. 2^8 of it, the largest v at
 // 2^14 .. 2^15, so that rounding up stays inside e4m3 (448) and e5m2 (57344).  A power of two costs no precision in a floating
 // format and makes every product with it exact.  16 lanes hold a block, eight elements each.
-__device__ inline float scale_float(uint32_t byte)          // 255: the block is not finite, every value of it reads as NaN
-{
-	return bits_float(byte << 23 | (byte == 255 ? 0x400000u : 0));
-}
+// The conversions of gfx950 take the scale as an f32 of which they use the exponent: byte << 23, and 255 reads as NaN.
+__device__ inline float scale_float(uint32_t byte) { return bits_float(byte << 23); }
 
-__device__ inline uint32_t block_max(uint32_t x)             // over the 16 lanes of a block
+template <class F> __device__ inline uint32_t row_reduce(uint32_t x, F f)            // over the 16 lanes of a block
 {
-#pragma unroll
-	for (int d = 1; d < 16; d <<= 1) x = max(x, (uint32_t) __shfl_xor((int) x, d, 16));
+	x = f(x, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, 0x128, 0xf, 0xf, false));     // rotated within the row by 8, 4, 2, 1
+	x = f(x, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, 0x124, 0xf, 0xf, false));
+	x = f(x, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, 0x122, 0xf, 0xf, false));
+	x = f(x, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, 0x121, 0xf, 0xf, false));
 	return x;
 }
 
@@ -187,92 +244,186 @@ __device__ inline uint32_t scale_byte(uint32_t top, int at)
 	return top >= 0x7f800000u ? 255u : (uint32_t) (e > 1 ? e : 1);
 }
 
-template <bool SECOND> __device__ inline u32x2 encode8(const float (&x)[kLane], uint32_t byte, uint32_t word)
+constexpr int kLane = 8;                                                     // elements of a block per lane
+
+template <bool SECOND> __device__ inline void encode(const float (&x)[kLane], uint32_t byte, uint32_t word, uint32_t (&c)[2])
 {
-	const float inv = byte == 255 ? 0.0f : bits_float((254u - byte) << 23);
-	u32x2 out = {0, 0};
-#pragma unroll
-	for (int j = 0; j < kLane; j++) {
-		float y = x[j] * inv;
-		const int r = (int) (word + j * kLaneStep);
-		// a second moment above zero stays above zero (the least code, 2^-16): m / (sqrt(0) + eps) would be a jump
-		if (SECOND) y = x[j] > 0 ? fmaxf(y, 0x1p-16f) : y;
-		const int c = SECOND ? __builtin_amdgcn_cvt_sr_bf8_f32(y, r, 0, 0) : __builtin_amdgcn_cvt_sr_fp8_f32(y, r, 0, 0);
-		out[j >> 2] |= (uint32_t) (c & 0xff) << (8 * (j & 3));
-	}
-	return out;
+	const float scale = scale_float(byte);
+	// a second moment above zero stays above zero (the least code, 2^-16): m / (sqrt(0) + eps) would be a jump
+	const float least = 0x1p-16f * scale;
+	int out[2] = {0, 0};
+	const auto one = [&](int j) {
+		const float y = SECOND ? (x[j] > 0 ? fmaxf(x[j], least) : x[j]) : x[j];
+		return y;
+	};
+#define TS_ENC(j, sel) out[(j) >> 2] = SECOND ? __builtin_amdgcn_cvt_scalef32_sr_bf8_f32(out[(j) >> 2], one(j), word + (j) * kLaneStep, scale, sel) \
+	: __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(out[(j) >> 2], one(j), word + (j) * kLaneStep, scale, sel)
+	TS_ENC(0, 0); TS_ENC(1, 1); TS_ENC(2, 2); TS_ENC(3, 3);
+	TS_ENC(4, 0); TS_ENC(5, 1); TS_ENC(6, 2); TS_ENC(7, 3);
+#undef TS_ENC
+	c[0] = (uint32_t) out[0];
+	c[1] = (uint32_t) out[1];
 }
 
-template <bool SECOND> __device__ inline void decode8(u32x2 c, float scale, float (&x)[kLane])
+template <bool SECOND> __device__ inline void decode(const uint32_t (&c)[2], float scale, float (&x)[kLane])
 {
 #pragma unroll
-	for (int j = 0; j < kLane; j += 2) {
-		const int w = (int) (c[j >> 2] >> (8 * (j & 2)));
-		const auto p = SECOND ? __builtin_amdgcn_cvt_pk_f32_bf8(w, false) : __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
-		x[j] = p[0] * scale;
-		x[j + 1] = p[1] * scale;
+	for (int k = 0; k < 2; k++) {
+		const auto p = SECOND ? __builtin_amdgcn_cvt_scalef32_pk_f32_bf8(c[k], scale, false) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[k], scale, false);
+		const auto q = SECOND ? __builtin_amdgcn_cvt_scalef32_pk_f32_bf8(c[k], scale, true) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[k], scale, true);
+		x[4 * k] = p[0]; x[4 * k + 1] = p[1]; x[4 * k + 2] = q[0]; x[4 * k + 3] = q[1];
 	}
 }
 
-template <int BITS> __global__ __launch_bounds__(kThreads) void k_adamw(const AdamwArgs a)
+// ---- the kernels -------------------------------------------------------------------------------------------------------------------
+struct Place {                                                               // a tensor as the lanes see it
+	void* param;
+	const void* grad;
+	uint64_t n, state;
+	float* master;
+	int ptype, gtype;
+	float decay;
+};
+__device__ inline Place place_of(const AdamwArgs& a, const TensorEntry& e, const Step& s)
 {
-	// a scale that is not finite: the step is rejected as a whole, nothing changes and nothing is counted
-	const float scale = a.grad_scale ? *a.grad_scale : 1.0f;
-	if (!(fabsf(scale) <= 3.402823466e38f)) return;
-	const long long t = a.count[0] + 1;
-	Step s = step_of(a, t);
-	s.scale = scale;
-	for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-		const int k = entry_of(a, tile);
-		const TensorEntry& e = a.entry[k];
-		const uint64_t n = e.info & kCountMask;
-		const int ptype = (int) (e.info >> 56) & 3, gtype = (int) (e.info >> 58) & 3;
-		const float decay = (e.info >> 60) & 1 ? 1.0f : s.decay;
-		const uint64_t i = (uint64_t) (tile - e.tile0) * kTile + threadIdx.x * kLane;
-		const uint64_t state = (a.block_base + e.block0) * kStateBlock;
-		float* master = a.master && ptype != T_F32 ? a.master + state : nullptr;
-		uint64_t word = 0;
-		if (BITS == 8 || s.stochastic) word = finalise(s.key + ((state + i) >> 3) * kGolden);
-		float g[kLane], w[kLane], m[kLane], v[kLane];
-		if (BITS == 32) {
-			if (i >= n) continue;
-			const f32x4* pm = reinterpret_cast<const f32x4*>(static_cast<float*>(a.m) + state + i);
-			const f32x4* pv = reinterpret_cast<const f32x4*>(static_cast<float*>(a.v) + state + i);
-			load8(e.grad, i, n, gtype, g);
-			load8(master ? master : e.param, i, n, master ? T_F32 : ptype, w);
-			const f32x4 m0 = pm[0], m1 = pm[1], v0 = pv[0], v1 = pv[1];
+	Place p;
+	p.param = e.param;
+	p.grad = e.grad;
+	p.n = e.info & kCountMask;
+	p.ptype = (int) (e.info >> 56) & 3;
+	p.gtype = (int) (e.info >> 58) & 3;
+	p.decay = (e.info >> 60) & 1 ? 1.0f : s.decay;
+	p.state = (a.block_base + e.block0) * kStateBlock;
+	p.master = a.master && p.ptype != T_F32 ? a.master + p.state : nullptr;
+	return p;
+}
+
+__device__ inline uint64_t word_of(const Step& s, uint64_t element) { return finalise(s.key + (element >> 3) * kGolden); }
+
+// moments in 32 bits: V elements per lane, U such groups in flight
+template <int V, int U> __device__ inline void chunk32(const AdamwArgs& a, const Step& s, const Place& p, uint64_t first)
+{
+	Raw<V> rg[U], rw[U], rm[U], rv[U];
+	float* const am = static_cast<float*>(a.m) + p.state;
+	float* const av = static_cast<float*>(a.v) + p.state;
+	const int wtype = p.master ? (int) T_F32 : p.ptype;
+	const void* const weights = p.master ? p.master : p.param;
 #pragma unroll
-			for (int j = 0; j < 4; j++) { m[j] = m0[j]; m[4 + j] = m1[j]; v[j] = v0[j]; v[4 + j] = v1[j]; }
+	for (int u = 0; u < U; u++) {
+		const uint64_t i = first + (u * kThreads + threadIdx.x) * V;
+		if (i >= p.n) continue;
+		load<V>(p.grad, i, p.n, p.gtype, rg[u]);
+		load<V>(weights, i, p.n, wtype, rw[u]);
+		fetch<V * 4, 16>(am + i, rm[u].w);
+		fetch<V * 4, 16>(av + i, rv[u].w);
+	}
 #pragma unroll
-			for (int j = 0; j < kLane; j++) update(s, decay, g[j] * s.scale, m[j], v[j], w[j]);
-			store8(static_cast<float*>(a.m) + state, i, n, m);
-			store8(static_cast<float*>(a.v) + state, i, n, v);
-		} else {
-			if ((i & ~(uint64_t) (kStateBlock - 1)) >= n) continue;      // whole blocks of 16 lanes leave together
-			const uint64_t b = (state + i) / kStateBlock;
-			u32x2* cm = reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.m) + state + i);
-			u32x2* cv = reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.v) + state + i);
-			load8(e.grad, i, n, gtype, g);
-			load8(master ? master : e.param, i, n, master ? T_F32 : ptype, w);
-			decode8<false>(*cm, scale_float(a.m_scale[b]), m);
-			decode8<true>(*cv, scale_float(a.v_scale[b]), v);
-			uint32_t tm = 0, tv = 0;                                    // bits of magnitudes order like the magnitudes, infinity and NaN last
+	for (int u = 0; u < U; u++) {
+		const uint64_t i = first + (u * kThreads + threadIdx.x) * V;
+		if (i >= p.n) continue;
+		float g[V], w[V], m[V], v[V];
+		widen<V>(rg[u], p.gtype, g);
+		widen<V>(rw[u], wtype, w);
+		uint32_t word = 0;
+		if (s.stochastic) word = (uint32_t) word_of(s, p.state + i) + (uint32_t) (i & 7) * kLaneStep;
 #pragma unroll
-			for (int j = 0; j < kLane; j++) {
-				update(s, decay, g[j] * s.scale, m[j], v[j], w[j]);
-				tm = max(tm, float_bits(m[j]) & 0x7fffffffu);
-				tv = max(tv, float_bits(v[j]) & 0x7fffffffu);
-			}
-			const uint32_t bm = scale_byte(block_max(tm), 7), bv = scale_byte(block_max(tv), 14);
-			*cm = encode8<false>(m, bm, (uint32_t) word);
-			*cv = encode8<true>(v, bv, (uint32_t) (word >> 32));
-			if ((threadIdx.x & 15) == 0) { a.m_scale[b] = (uint8_t) bm; a.v_scale[b] = (uint8_t) bv; }
-			if (i >= n) continue;
+		for (int j = 0; j < V; j++) {
+			m[j] = bits_float(rm[u].w[j]);
+			v[j] = bits_float(rv[u].w[j]);
+			update(s, p.decay, g[j] * s.scale, m[j], v[j], w[j]);
 		}
-		put_weights(a, s, e.param, i, n, ptype, master, w, (uint32_t) word);
+		store32<V>(am, i, p.n, m);
+		store32<V>(av, i, p.n, v);
+		put_weights<V>(s, p.param, i, p.n, p.ptype, p.master, w, word);
 	}
-	// the last workgroup to arrive counts the step: by then every other one has read the counter
-	if (a.last && threadIdx.x == 0) {
+}
+
+// moments in 8 bits: 16 lanes of eight elements are a block, U such groups in flight
+template <int U> __device__ inline void chunk8(const AdamwArgs& a, const Step& s, const Place& p, uint64_t first)
+{
+	Raw<kLane> rg[U], rw[U];
+	uint32_t cm[U][2], cv[U][2];
+	uint8_t sm[U], sv[U];
+	uint8_t* const am = static_cast<uint8_t*>(a.m) + p.state;
+	uint8_t* const av = static_cast<uint8_t*>(a.v) + p.state;
+	uint8_t* const bm = a.m_scale + p.state / kStateBlock;
+	uint8_t* const bv = a.v_scale + p.state / kStateBlock;
+	const int wtype = p.master ? (int) T_F32 : p.ptype;
+	const void* const weights = p.master ? p.master : p.param;
+#pragma unroll
+	for (int u = 0; u < U; u++) {
+		const uint64_t i = first + (u * kThreads + threadIdx.x) * kLane;
+		if ((i & ~(uint64_t) (kStateBlock - 1)) >= p.n) continue;            // whole blocks of 16 lanes leave together
+		sm[u] = bm[i / kStateBlock];
+		sv[u] = bv[i / kStateBlock];
+		load<kLane>(p.grad, i, p.n, p.gtype, rg[u]);
+		load<kLane>(weights, i, p.n, wtype, rw[u]);
+		fetch<8, 8>(am + i, cm[u]);
+		fetch<8, 8>(av + i, cv[u]);
+	}
+#pragma unroll
+	for (int u = 0; u < U; u++) {
+		const uint64_t i = first + (u * kThreads + threadIdx.x) * kLane;
+		if ((i & ~(uint64_t) (kStateBlock - 1)) >= p.n) continue;
+		float g[kLane], w[kLane], m[kLane], v[kLane];
+		widen<kLane>(rg[u], p.gtype, g);
+		widen<kLane>(rw[u], wtype, w);
+		decode<false>(cm[u], scale_float(sm[u]), m);
+		decode<true>(cv[u], scale_float(sv[u]), v);
+		const uint64_t word = word_of(s, p.state + i);
+		// Bits of magnitudes order like the magnitudes, infinity and NaN last.  The first moment's maximum passes over NaN; but
+		// where m is NaN so is v, of the same element.
+		float tm = 0;
+		uint32_t tv = 0;
+#pragma unroll
+		for (int j = 0; j < kLane; j++) {
+			update(s, p.decay, g[j] * s.scale, m[j], v[j], w[j]);
+			tm = fmaxf(tm, fabsf(m[j]));
+			tv = max(tv, float_bits(v[j]) & 0x7fffffffu);
+		}
+		tv = row_reduce(tv, [](uint32_t x, uint32_t y) { return max(x, y); });
+		if (tv >= 0x7f800000u) {
+#pragma unroll
+			for (int j = 0; j < kLane; j++)
+				if (m[j] != m[j]) tm = __builtin_inff();
+		}
+		const uint32_t om = scale_byte(row_reduce(float_bits(tm), [](uint32_t x, uint32_t y) { return max(x, y); }), 7), ov = scale_byte(tv, 14);
+		uint32_t c[2];
+		encode<false>(m, om, (uint32_t) word, c);
+		put<8, 8>(am + i, c);
+		encode<true>(v, ov, (uint32_t) (word >> 32), c);
+		put<8, 8>(av + i, c);
+		if ((threadIdx.x & 15) == 0) { bm[i / kStateBlock] = (uint8_t) om; bv[i / kStateBlock] = (uint8_t) ov; }
+		if (i < p.n) put_weights<kLane>(s, p.param, i, p.n, p.ptype, p.master, w, (uint32_t) word);
+	}
+}
+
+// The step's numbers once for all workgroups: a kernel of one lane in front of the step.  They are a few hundred cycles of f64, and counting
+// the step here needs no workgroup to wait for the others; where every workgroup does it and arrives at one counter, arrivals
+// take 6.5 ns each, one after the other.
+__global__ void k_adamw_begin(const AdamwArgs a)
+{
+	const long long t = a.count[0] + 1;
+	const Step s = step_of(a, t);
+	*a.step = s;
+	if (s.go) a.count[0] = t;
+}
+
+// TILE elements at a time; ALONE: a few workgroups form the step's numbers themselves, and the last to arrive counts the step
+template <int BITS, int TILE, bool ALONE> __global__ __launch_bounds__(kThreads) void k_adamw(const AdamwArgs a)
+{
+	const long long t = ALONE ? a.count[0] + 1 : 0;
+	const Step s = ALONE ? step_of(a, t) : *a.step;
+	if (!s.go) return;
+	Cursor<AdamwArgs> cursor(a, blockIdx.x);
+	for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+		const TensorEntry& e = cursor.at(tile);
+		const Place p = place_of(a, e, s);
+		const uint64_t first = (uint64_t) (tile - e.tile0) * TILE;
+		if (BITS == 32) chunk32<4, TILE / kThreads / 4>(a, s, p, first);
+		else chunk8<TILE / kThreads / kLane>(a, s, p, first);
+	}
+	if (ALONE && threadIdx.x == 0) {                    // by the last arrival every other workgroup has read the counter
 		unsigned long long* arrived = reinterpret_cast<unsigned long long*>(a.count + 1);
 		if (__hip_atomic_fetch_add(arrived, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
 			__hip_atomic_store(arrived, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -303,18 +454,27 @@ __device__ inline void verdict(double sum, double grad_scale, double max_norm, f
 	out[1] = !finite ? __builtin_nanf("") : (float) (norm > max_norm ? grad_scale * (max_norm / norm) : grad_scale);
 }
 
-__global__ __launch_bounds__(kThreads) void k_norm(const NormArgs a)
+template <int TILE> __global__ __launch_bounds__(kThreads) void k_norm(const NormArgs a)
 {
+	constexpr int V = 8, U = TILE / kThreads / V;
 	double sum = 0;
+	Cursor<NormArgs> cursor(a, blockIdx.x);
 	for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-		const TensorEntry& e = a.entry[entry_of(a, tile)];
-		const uint64_t n = e.info & kCountMask;
-		const uint64_t i = (uint64_t) (tile - e.tile0) * kTile + threadIdx.x * kLane;
-		if (i >= n) continue;
-		float g[kLane];
-		load8(e.grad, i, n, (int) (e.info >> 58) & 3, g);
+		const TensorEntry& e = cursor.at(tile);
+		const uint64_t n = e.info & kCountMask, first = (uint64_t) (tile - e.tile0) * TILE + threadIdx.x * V;
+		const int type = (int) (e.info >> 58) & 3;
+		Raw<V> r[U];
 #pragma unroll
-		for (int j = 0; j < kLane; j++) sum = fma((double) g[j], (double) g[j], sum);
+		for (int u = 0; u < U; u++)
+			if (first + u * kThreads * V < n) load<V>(e.grad, first + u * kThreads * V, n, type, r[u]);
+#pragma unroll
+		for (int u = 0; u < U; u++) {
+			if (first + u * kThreads * V >= n) continue;
+			float g[V];
+			widen<V>(r[u], type, g);
+#pragma unroll
+			for (int j = 0; j < V; j++) sum = fma((double) g[j], (double) g[j], sum);
+		}
 	}
 	sum = block_sum(sum);
 	if (threadIdx.x) return;
@@ -336,12 +496,22 @@ __global__ void k_norm_verdict(const double* sum, double grad_scale, double max_
 
 }  // namespace
 
-void launch_adamw(hipStream_t st, int bits, int grid, const AdamwArgs& a)
+void launch_adamw_begin(hipStream_t st, const AdamwArgs& a) { k_adamw_begin<<<1, 1, 0, st>>>(a); }
+void launch_adamw(hipStream_t st, int bits, int tile, int grid, const AdamwArgs& a)
 {
-	if (bits == 8) k_adamw<8><<<grid, kThreads, 0, st>>>(a);
-	else k_adamw<32><<<grid, kThreads, 0, st>>>(a);
+	if (bits == 8) {
+		if (a.step) tile == kTileSmall ? k_adamw<8, kTileSmall, false><<<grid, kThreads, 0, st>>>(a) : k_adamw<8, kTile8, false><<<grid, kThreads, 0, st>>>(a);
+		else k_adamw<8, kTileSmall, true><<<grid, kThreads, 0, st>>>(a);
+	} else {
+		if (a.step) tile == kTileSmall ? k_adamw<32, kTileSmall, false><<<grid, kThreads, 0, st>>>(a) : k_adamw<32, kTile32, false><<<grid, kThreads, 0, st>>>(a);
+		else k_adamw<32, kTileSmall, true><<<grid, kThreads, 0, st>>>(a);
+	}
 }
-void launch_norm(hipStream_t st, int grid, const NormArgs& a) { k_norm<<<grid, kThreads, 0, st>>>(a); }
+void launch_norm(hipStream_t st, int tile, int grid, const NormArgs& a)
+{
+	if (tile == kTileSmall) k_norm<kTileSmall><<<grid, kThreads, 0, st>>>(a);
+	else k_norm<kTile8><<<grid, kThreads, 0, st>>>(a);
+}
 void launch_norm_sum(hipStream_t st, double* part, int count, double grad_scale, double max_norm, float* out)
 {
 	k_norm_sum<<<1, kThreads, 0, st>>>(part, count, grad_scale, max_norm, out);

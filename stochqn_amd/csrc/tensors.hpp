@@ -9,7 +9,9 @@
 namespace sqn {
 
 constexpr int kStateBlock = 128;     // elements that share the scale of an 8-bit moment; every tensor's state starts at a multiple of it
-constexpr int kTile = 2048;          // elements a workgroup of 256 threads takes at a time, eight per lane
+constexpr int kTileSmall = 2048;     // elements a workgroup of 256 threads takes at a time: of a few tensors that would not fill the card otherwise,
+constexpr int kTile32 = 4096;        // and of many, with moments in 32 bits,
+constexpr int kTile8 = 8192;         // in 8 bits, and for the norm
 constexpr int kEntries = 112;        // tensors per launch: the table travels in the kernel's arguments (32 B each, 4 KB in all)
 
 enum TensorType { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
@@ -20,7 +22,7 @@ struct TensorEntry {
 	void* param;
 	const void* grad;
 	uint64_t info;
-	uint32_t tile0;              // first tile of this launch that is the tensor's
+	uint32_t tile0;              // first tile of this launch that is the tensor's (tiles of LaunchShape::tile elements)
 	uint32_t block0;             // first block of kStateBlock elements of its state, counted from AdamwArgs::block_base
 };
 constexpr uint64_t kCountMask = (1ull << 56) - 1;
@@ -28,6 +30,21 @@ inline uint64_t entry_info(size_t count, int ptype, int gtype, bool no_decay)
 {
 	return (uint64_t) count | (uint64_t) ptype << 56 | (uint64_t) gtype << 58 | (uint64_t) no_decay << 60;
 }
+
+// How a list is cut up: one rule for every call on it, by its sizes alone.
+struct LaunchShape {
+	int tile;                    // elements of a tile
+	int grid;                    // most workgroups
+};
+
+// What is the same for every element of a step (tensors.hip: step_of)
+struct Step {
+	float scale, b1, b2, a1, a2, decay, rate, root, eps;
+	int stochastic, careful, go;                         // go = 0: rejected
+	uint64_t key;
+};
+constexpr size_t kStepBytes = 64;
+static_assert(sizeof(Step) <= kStepBytes, "the caller's work area");
 
 struct AdamwArgs {
 	TensorEntry entry[kEntries];
@@ -38,12 +55,12 @@ struct AdamwArgs {
 	void *m, *v;                 // f32[state] or codes [state]
 	uint8_t *m_scale, *v_scale;  // [state / kStateBlock], 8-bit moments only
 	long long* count;            // [0] steps taken, [1] workgroups that have arrived (zero between steps)
+	Step* step;                  // where launch_adamw_begin left the step's numbers; NULL: every workgroup forms them
 	const float* grad_scale;     // what every gradient is multiplied with; NULL = 1
 	const float* step_size_dev;  // NULL: step_size
 	double step_size, beta1, beta2, weight_decay;
 	float eps;
 	uint64_t seed;
-	int last;                    // the launch that counts the step
 	int stochastic;              // bf16 parameters without f32 weights beside them are rounded stochastically
 };
 static_assert(sizeof(AdamwArgs) <= 4096, "kernel arguments");
@@ -58,8 +75,9 @@ struct NormArgs {
 };
 static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
 
-void launch_adamw(hipStream_t st, int bits, int grid, const AdamwArgs& a);
-void launch_norm(hipStream_t st, int grid, const NormArgs& a);
+void launch_adamw_begin(hipStream_t st, const AdamwArgs& a);      // the step's numbers -> a.step, and the step is counted
+void launch_adamw(hipStream_t st, int bits, int tile, int grid, const AdamwArgs& a);
+void launch_norm(hipStream_t st, int tile, int grid, const NormArgs& a);
 // part[0] <- the sum of part[1 .. count] (in a fixed order); with `out` also the verdict
 void launch_norm_sum(hipStream_t st, double* part, int count, double grad_scale, double max_norm, float* out);
 // the verdict of a sum of squares that is final: out[0] the norm, out[1] the coefficient

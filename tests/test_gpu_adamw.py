@@ -539,7 +539,7 @@ def test_refusals_of_the_c_entries(capfd):
     n = 1000
     p = torch.zeros(n, device="cuda")
     st = [torch.zeros(1024, device="cuda") for _ in range(3)]
-    count = torch.zeros(2, dtype=torch.int64, device="cuda")
+    count, work = torch.zeros(2, dtype=torch.int64, device="cuda"), torch.zeros(8, dtype=torch.int64, device="cuda")
     one = lambda ptr, size=n, type=0: lib.stochqn_hip_tensors_create(1, (C.c_void_p * 1)(ptr), (C.c_size_t * 1)(size), (C.c_int * 1)(type))
     hostmem = np.zeros(n, dtype=np.float32)
     for bad in (dict(ptr=hostmem.ctypes.data), dict(ptr=None), dict(ptr=p.data_ptr() + 2), dict(ptr=p.data_ptr(), size=2 ** 40), dict(ptr=p.data_ptr(), size=2 ** 42),
@@ -549,13 +549,13 @@ def test_refusals_of_the_c_entries(capfd):
     params = one(p.data_ptr())
     grads = one(st[2].data_ptr())
     good = dict(beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, state_bits=32, stochastic=0, seed=0, m=st[0].data_ptr(), v=st[1].data_ptr(),
-                count=count.data_ptr())
+                count=count.data_ptr(), work=work.data_ptr())
 
     def make(**kw):
         s = _Setup(**dict(good, **kw))
         return lib.stochqn_hip_adamw_create(params, C.byref(s))
     for bad in (dict(beta1=1.0), dict(eps=0.0), dict(eps=math.inf), dict(weight_decay=math.inf), dict(state_bits=4), dict(state_bits=8), dict(m=None),
-                dict(m=st[0].data_ptr() + 4), dict(m=hostmem.ctypes.data), dict(v=st[0].data_ptr()), dict(m=p.data_ptr()), dict(count=None),
+                dict(m=st[0].data_ptr() + 4), dict(m=hostmem.ctypes.data), dict(v=st[0].data_ptr()), dict(m=p.data_ptr()), dict(count=None), dict(work=None), dict(work=count.data_ptr()),
                 dict(count=st[0].data_ptr() + 8), dict(m_scale=st[2].data_ptr()), dict(stochastic=1, master=st[2].data_ptr())):
         assert not make(**bad), bad
     opt = make()
