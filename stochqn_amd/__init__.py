@@ -62,7 +62,14 @@ def lib(use_float=False):
     return _bound[key]
 
 
-from .adamw import AdamW_free, TensorList  # noqa: E402
 from .free import oLBFGS_free, SQN_free, adaQN_free  # noqa: E402
 
 __all__ = ["lib", "cdll", "LIB_PATH", "oLBFGS_free", "SQN_free", "adaQN_free", "AdamW_free", "TensorList"]
+
+
+def __getattr__(name):
+    """The objects over torch tensors are imported when they are asked for: the rest does without torch."""
+    if name in ("AdamW_free", "TensorList"):
+        from . import adamw
+        return getattr(adamw, name)
+    raise AttributeError("module 'stochqn_amd' has no attribute '%s'" % name)

@@ -8,6 +8,8 @@ with it, without a synchronisation, and may be captured into a graph.
 import ctypes as C
 import math
 
+import torch
+
 BLOCK = 128                     # elements that share a scale; every tensor's state starts at a multiple of it
 
 
@@ -44,13 +46,16 @@ def _library():
 
 
 def _types():
-    import torch
     return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _stream(index):
+    """The current torch stream of a device, as the address that the library takes (torch.cuda.current_stream makes an object: 2 us)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _scalar(t, device, what):
     """Address of a device tensor of one float32 (None: none)."""
-    import torch
     if t is None:
         return None
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
@@ -71,36 +76,39 @@ class TensorList:
         types = _types()
         if not self.tensors:
             raise ValueError("no tensors.")
-        self.device = getattr(self.tensors[0], "device", None)
-        for t in self.tensors:
-            if getattr(t, "dtype", None) not in types:
-                raise ValueError("tensors have to be float32, bfloat16 or float16.")
-        self._check(self.tensors)
+        if not all(getattr(t, "dtype", None) in types for t in self.tensors):
+            raise ValueError("tensors have to be float32, bfloat16 or float16.")
         n = len(self.tensors)
+        self.device = self.tensors[0].device
+        self._index = self.tensors[0].get_device()
         self.sizes = [t.numel() for t in self.tensors]
         self.dtypes = [t.dtype for t in self.tensors]
+        self._at = self._addresses(self.tensors)
         self._lib = _library()
-        self._at = [t.data_ptr() for t in self.tensors]
         self._handle = self._lib.stochqn_hip_tensors_create(n, (C.c_void_p * n)(*self._at), (C.c_size_t * n)(*self.sizes),
                                                             (C.c_int * n)(*[types[d] for d in self.dtypes]))
         if not self._handle:
             raise ValueError("the library refused the tensors (its reason is on stderr).")
         self._work = self._lib.stochqn_hip_tensors_norm_work(self._handle)
 
-    def _check(self, tensors):
-        for t in tensors:
-            if not t.is_cuda or t.device != self.device:
+    def _addresses(self, tensors):
+        at = []
+        for t, n, dtype in zip(tensors, self.sizes, self.dtypes):
+            if t.numel() != n or t.dtype != dtype:
+                raise ValueError("the tensors have other sizes or types than the list's.")
+            if t.get_device() != self._index or not t.is_cuda:
                 raise ValueError("tensors have to be on one GPU.")
             if not t.is_contiguous():
                 raise ValueError("tensors have to be contiguous.")
+            at.append(t.data_ptr())
+        return at
 
     def rebind(self, tensors):
         """Other tensors of the same sizes and types take the place of the list's (new gradients of the same parameters)."""
         tensors = list(tensors)
-        if [t.numel() for t in tensors] != self.sizes or [t.dtype for t in tensors] != self.dtypes:
+        if len(tensors) != len(self.sizes):
             raise ValueError("the tensors have other sizes or types than the list's.")
-        self._check(tensors)
-        at = [t.data_ptr() for t in tensors]
+        at = self._addresses(tensors)
         if at != self._at:
             if self._lib.stochqn_hip_tensors_rebind(self._handle, (C.c_void_p * len(at))(*at)) != 0:
                 raise ValueError("the library refused the tensors (its reason is on stderr).")
@@ -114,7 +122,6 @@ class TensorList:
         """A float32 tensor of two elements on the device: the norm over all tensors times `grad_scale` (1 / loss scale), and the factor
         that brings the gradients to a norm of at most `max_norm` -- NaN if the norm is not finite, which makes the step that takes it
         (`run_optimizer(..., grad_scale=out[1:])`) a rejected one.  With a communicator installed: over all ranks' tensors."""
-        import torch
         max_norm = math.inf if max_norm is None else float(max_norm)
         if not max_norm > 0 or not math.isfinite(grad_scale):
             raise ValueError("'max_norm' has to be positive and 'grad_scale' finite.")
@@ -123,8 +130,7 @@ class TensorList:
         elif out.dtype != torch.float32 or out.shape != (2,) or out.device != self.device or not out.is_contiguous():
             raise ValueError("'out' has to be a float32 tensor of two elements on %s." % self.device)
         work = torch.empty(self._work, dtype=torch.float64, device=self.device)      # of this call alone: two streams, or two graphs, share none
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        if self._lib.stochqn_hip_tensors_norm(self._handle, grad_scale, max_norm, out.data_ptr(), work.data_ptr(), stream) != 0:
+        if self._lib.stochqn_hip_tensors_norm(self._handle, grad_scale, max_norm, out.data_ptr(), work.data_ptr(), _stream(self._index)) != 0:
             raise RuntimeError("stochqn_hip_tensors_norm failed (its reason is on stderr).")
         return out
 
@@ -149,7 +155,6 @@ class AdamW_free:
 
     def __init__(self, params, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, state_bits=32, master=False, stochastic=False,
                  decay=None, seed=0):
-        import torch
         assert 0 <= beta1 < 1 and 0 <= beta2 < 1
         assert 2.0 ** -126 <= eps < 3e38 and math.isfinite(weight_decay)
         assert state_bits in (8, 32)
@@ -174,7 +179,7 @@ class AdamW_free:
             byte = lambda n, dtype: zeros(n, torch.uint8).view(dtype)
             self.m, self.v = byte(total, torch.float8_e4m3fn), byte(total, torch.float8_e5m2)
             self.m_scale, self.v_scale = byte(total // BLOCK, torch.float8_e8m0fnu), byte(total // BLOCK, torch.float8_e8m0fnu)
-        self.count, self._work = zeros(2, torch.int64), zeros(8, torch.int64)
+        self.count, self._work = zeros(2, torch.int64), zeros(512, torch.int64)
         self.master = None
         if master:
             self.master = zeros(total, torch.float32)
@@ -199,21 +204,18 @@ class AdamW_free:
             self.gradient, self._own_list = gradient, False
             return
         gradient = list(gradient)
-        if [t.numel() for t in gradient] != self.params.sizes:
-            raise ValueError("the gradients have other sizes than the parameters.")
         if self._own_list and [t.dtype for t in gradient] == self.gradient.dtypes:
             self.gradient.rebind(gradient)
             return
         new = TensorList(gradient)
-        if new.device != self.params.device:
-            raise ValueError("the gradients are on another device than the parameters.")
+        if new.sizes != self.params.sizes or new.device != self.params.device:
+            raise ValueError("the gradients have other sizes or another device than the parameters.")
         self.gradient, self._own_list = new, True
 
     def run_optimizer(self, step_size, grad_scale=None):
         """One step.  step_size: a number, or a float32 tensor of one element on the device (schedules in a captured graph).  grad_scale: None,
         or such a tensor that every gradient is multiplied with (`TensorList.norm(...)[1:]`); if it is not finite the step is rejected:
         no weight, no moment and no count changes."""
-        import torch
         if self.gradient is None:
             raise ValueError("no gradient: call update_gradient first.")
         dev = self.params.device
@@ -223,8 +225,7 @@ class AdamW_free:
         elif not math.isfinite(step_size):
             raise ValueError("'step_size' is not finite.")
         scale = _scalar(grad_scale, dev, "grad_scale")
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        if self._lib.stochqn_hip_adamw_step(self._handle, self.gradient._handle, step_size, step_dev, scale, stream) != 0:
+        if self._lib.stochqn_hip_adamw_step(self._handle, self.gradient._handle, step_size, step_dev, scale, _stream(dev.index)) != 0:
             raise RuntimeError("stochqn_hip_adamw_step failed (its reason is on stderr).")
 
     def moments(self, i):

@@ -21,9 +21,6 @@ namespace {
 // Most workgroups per compute unit (measured at 1.28e9 elements): 32-bit moments 4, 8 and 16 alike; 8-bit moments 2.53 ms with 8, 2.46 with 16,
 // 2.41 with 32; the norm 466 us with 4, 380 with 8, 384 with 16.
 constexpr int kPerUnit32 = 8, kPerUnit8 = 32, kPerUnitNorm = 8;
-// Up to this many small tiles a step is one launch whose workgroups form its numbers themselves and count it by arrivals, 6.5 ns each;
-// beyond, a kernel in front does (3.5 us in a stream of steps): 7.6 against 11.2 us a step of 57 tiles.
-constexpr uint64_t kAloneTiles = 256;
 
 struct Range { const char* at; size_t bytes; };                              // of device memory
 bool before(const Range& a, const Range& b) { return a.at < b.at; }
@@ -71,12 +68,15 @@ void check_aligned(const void* p, size_t to, const char* what)
 
 uint64_t tiles_of(size_t n, int tile) { return (n + tile - 1) / tile; }
 
-// Large tiles keep more loads of a lane in flight; a list that has fewer of them than two for each compute unit is cut into small ones.
-LaunchShape shape_of(const std::vector<Item>& items, int units, int large, int per_unit)
+// Large tiles keep more loads of a lane in flight; a list with fewer than `few` of them for each compute unit is cut into small ones.  Measured at
+// 7.7e6 elements: the step with 8-bit moments 21.1 us small, 24.2 large (3.7 a unit), with 32-bit moments 44.8 and 46.3 (7.4 a unit); the
+// norm, whose partial sums have to be added up, 12.6 and 11.0.
+constexpr int kFewStep = 8, kFewNorm = 2;
+LaunchShape shape_of(const std::vector<Item>& items, int units, int large, int few, int per_unit)
 {
 	uint64_t tiles = 0;
 	for (const Item& it : items) tiles += tiles_of(it.n, large);
-	return {tiles < 2 * (uint64_t) units ? kTileSmall : large, units * per_unit};
+	return {tiles < few * (uint64_t) units ? kTileSmall : large, units * per_unit};
 }
 
 size_t blocks_of(size_t n) { return (n + kStateBlock - 1) / kStateBlock; }
@@ -171,7 +171,7 @@ template <class Fill, class Fire> void for_launches(const std::vector<Item>& ite
 		if (!items[i].n) continue;
 		const uint64_t mine = tiles_of(items[i].n, tile);
 		if (used == kEntries || (used && tiles + mine > 0x7fffffffu)) {
-			fire(used, (uint32_t) tiles);
+			fire(used, (uint32_t) tiles, false);
 			used = 0;
 			tiles = 0;
 		}
@@ -180,7 +180,7 @@ template <class Fill, class Fire> void for_launches(const std::vector<Item>& ite
 		used++;
 		tiles += mine;
 	}
-	fire(used, (uint32_t) tiles);
+	fire(used, (uint32_t) tiles, true);
 }
 
 }  // namespace
@@ -201,7 +201,7 @@ stochqn_hip_tensors* stochqn_hip_tensors_create(int count, void* const ptr[], co
 		set_items(t->items, t->device, ptr);
 		if (t->device < 0 && hipGetDevice(&t->device) != hipSuccess) refuse("no current device");
 		t->units = units_of(t->device);
-		t->norm = shape_of(t->items, t->units, kTile8, kPerUnitNorm);
+		t->norm = shape_of(t->items, t->units, kTile8, kFewNorm, kPerUnitNorm);
 		t->version = ++g_versions;
 		return t.release();
 	});
@@ -237,7 +237,7 @@ size_t stochqn_hip_tensors_norm_work(const stochqn_hip_tensors* t)
 	if (!t) return 0;
 	size_t parts = 0;
 	TensorEntry table[kEntries];
-	for_launches(t->items, t->norm.tile, table, [](size_t, int) {}, [&](int, uint32_t tiles) { parts += std::min<size_t>(tiles, t->norm.grid); });
+	for_launches(t->items, t->norm.tile, table, [](size_t, int) {}, [&](int, uint32_t tiles, bool) { parts += std::min<size_t>(tiles, t->norm.grid); });
 	return 1 + parts;
 }
 
@@ -256,24 +256,25 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors* t, double grad_scale, double m
 		OnDevice on(device);
 		hipStream_t st = check_stream(hip_stream, device);
 		const bool reduced = comm_nranks() > 1;
-		NormArgs a{};
+		Table<NormArgs, kEntries> table;
+		NormArgs& a = table.a;
 		a.grad_scale = grad_scale;
 		a.max_norm = max_norm;
 		int parts = 0, launches = 0;
 		bool done = false;
-		for_launches(t->items, t->norm.tile, a.entry,
+		for_launches(t->items, t->norm.tile, table.entry,
 			[&](size_t i, int k) {
-				a.entry[k].grad = t->items[i].p;
-				a.entry[k].info = entry_info(t->items[i].n, 0, t->items[i].type, false);
+				table.entry[k].grad = t->items[i].p;
+				table.entry[k].info = entry_info(t->items[i].n, 0, t->items[i].type, false);
 			},
-			[&](int used, uint32_t tiles) {
+			[&](int used, uint32_t tiles, bool) {
 				a.entries = used;
 				a.tiles = tiles;
 				a.part = work + 1 + parts;
 				done = tiles <= 1 && !launches && !reduced;             // one workgroup sees everything: it finishes
 				a.out = done ? out : nullptr;
 				const int grid = (int) std::min<size_t>(done ? 1 : tiles, t->norm.grid);
-				if (grid) launch_norm(st, t->norm.tile, grid, a);
+				if (grid) launch_norm(st, t->norm.tile, grid, table);
 				parts += grid;
 				launches++;
 			});
@@ -301,7 +302,7 @@ stochqn_hip_adamw* stochqn_hip_adamw_create(stochqn_hip_tensors* params, const s
 		std::lock_guard<std::mutex> lk(params->mu);
 		o->items = params->items;
 		o->device = params->device;
-		o->shape = s.state_bits == 8 ? shape_of(o->items, params->units, kTile8, kPerUnit8) : shape_of(o->items, params->units, kTile32, kPerUnit32);
+		o->shape = s.state_bits == 8 ? shape_of(o->items, params->units, kTile8, kFewStep, kPerUnit8) : shape_of(o->items, params->units, kTile32, kFewStep, kPerUnit32);
 		o->s = s;
 		size_t blocks = 0;
 		for (size_t i = 0; i < o->items.size(); i++) {
@@ -327,7 +328,7 @@ stochqn_hip_adamw* stochqn_hip_adamw_create(stochqn_hip_tensors* params, const s
 		array(s.v_scale, s.state_bits == 8 ? blocks : 0, 1, "v_scale");
 		array(s.master, state * sizeof(float), 16, "master");
 		array(s.count, 2 * sizeof(long long), 8, "count");
-		array(s.work, kStepBytes, 8, "work");
+		array(s.work, kGates * kGateStride, 8, "work");
 		std::sort(o->written.begin(), o->written.end(), before);
 		for (size_t i = 1; i < o->written.size(); i++)
 			if (o->written[i - 1].at + o->written[i - 1].bytes > o->written[i].at) refuse("two arrays that the step writes overlap");
@@ -365,13 +366,15 @@ int stochqn_hip_adamw_step(stochqn_hip_adamw* o, stochqn_hip_tensors* grads, dou
 		OnDevice on(o->device);
 		hipStream_t st = check_stream(hip_stream, o->device);
 		const stochqn_hip_adamw_setup& s = o->s;
-		AdamwArgs a{};
+		Table<AdamwArgs, kEntries> table;
+		AdamwArgs& a = table.a;
 		a.master = s.master;
 		a.m = s.m;
 		a.v = s.v;
 		a.m_scale = s.m_scale;
 		a.v_scale = s.v_scale;
 		a.count = s.count;
+		a.gates = static_cast<char*>(s.work);
 		a.grad_scale = grad_scale;
 		a.step_size_dev = step_size_dev;
 		a.step_size = step_size;
@@ -381,26 +384,20 @@ int stochqn_hip_adamw_step(stochqn_hip_adamw* o, stochqn_hip_tensors* grads, dou
 		a.eps = (float) s.eps;
 		a.seed = s.seed;
 		a.stochastic = s.stochastic;
-		// few workgroups, one launch: they form the step's numbers themselves; else a kernel in front does
-		uint64_t all = 0;
-		for (const Item& it : o->items) all += tiles_of(it.n, o->shape.tile);
-		const bool alone = o->items.size() <= (size_t) kEntries && all <= kAloneTiles && o->shape.tile == kTileSmall;
-		a.step = alone ? nullptr : static_cast<Step*>(s.work);
-		if (!alone) launch_adamw_begin(st, a);
-		for_launches(o->items, o->shape.tile, a.entry,
+		for_launches(o->items, o->shape.tile, table.entry,
 			[&](size_t i, int k) {
-				TensorEntry& e = a.entry[k];
+				TensorEntry& e = table.entry[k];
 				if (!k) a.block_base = o->block[i];
 				e.param = o->items[i].p;
 				e.grad = g[i].p;
 				e.info = entry_info(g[i].n, o->items[i].type, g[i].type, o->no_decay[i]);
 				e.block0 = (uint32_t) (o->block[i] - a.block_base);
 			},
-			[&](int used, uint32_t tiles) {
+			[&](int used, uint32_t tiles, bool last) {
 				a.entries = used;
 				a.tiles = tiles;
-				const int grid = (int) std::min<size_t>(alone ? std::max<uint32_t>(tiles, 1) : tiles, o->shape.grid);
-				if (grid) launch_adamw(st, s.state_bits, o->shape.tile, grid, a);
+				a.last = last;
+				launch_adamw(st, s.state_bits, o->shape.tile, (int) std::min<size_t>(std::max<uint32_t>(tiles, 1), o->shape.grid), table);
 			});
 		return launched();
 	});

@@ -119,25 +119,25 @@ template <int V> __device__ inline void store16(uint16_t* base, uint64_t i, uint
 }
 
 // the tensor that a workgroup is at: found by bisection once, then followed (its tiles come in rising order)
-template <class Args> struct Cursor {
-	const Args& a;
+template <class T> struct Cursor {
+	const T& t;
 	int k;
 	uint32_t next;
-	__device__ Cursor(const Args& args, uint32_t tile) : a(args)
+	__device__ Cursor(const T& table, uint32_t tile) : t(table)
 	{
-		int lo = 0, hi = a.entries;
+		int lo = 0, hi = t.a.entries;
 		while (hi - lo > 1) {
 			const int mid = (lo + hi) >> 1;
-			if (a.entry[mid].tile0 <= tile) lo = mid; else hi = mid;
+			if (t.entry[mid].tile0 <= tile) lo = mid; else hi = mid;
 		}
 		k = lo;
 		next = end();
 	}
-	__device__ uint32_t end() const { return k + 1 < a.entries ? a.entry[k + 1].tile0 : 0xffffffffu; }
+	__device__ uint32_t end() const { return k + 1 < t.a.entries ? t.entry[k + 1].tile0 : 0xffffffffu; }
 	__device__ const TensorEntry& at(uint32_t tile)
 	{
 		while (tile >= next) { k++; next = end(); }
-		return a.entry[k];
+		return t.entry[k];
 	}
 };
 
@@ -158,6 +158,12 @@ __device__ inline uint64_t finalise(uint64_t z)
 }
 
 // ---- what is the same for every element of a step ---------------------------------------------------------------------------------
+struct Step {
+	float scale, b1, b2, a1, a2, decay, rate, root, eps;
+	uint64_t key;
+	bool go, stochastic, careful;
+};
+
 __device__ inline Step step_of(const AdamwArgs& a, long long t)
 {
 	Step s{};
@@ -282,9 +288,11 @@ struct Place {                                                               // 
 	uint64_t n, state;
 	float* master;
 	int ptype, gtype;
-	float decay;
+	bool decays;
+	__device__ int wtype() const { return master ? (int) T_F32 : ptype; }
+	__device__ const void* weights() const { return master ? master : param; }
 };
-__device__ inline Place place_of(const AdamwArgs& a, const TensorEntry& e, const Step& s)
+__device__ inline Place place_of(const AdamwArgs& a, const TensorEntry& e)
 {
 	Place p;
 	p.param = e.param;
@@ -292,7 +300,7 @@ __device__ inline Place place_of(const AdamwArgs& a, const TensorEntry& e, const
 	p.n = e.info & kCountMask;
 	p.ptype = (int) (e.info >> 56) & 3;
 	p.gtype = (int) (e.info >> 58) & 3;
-	p.decay = (e.info >> 60) & 1 ? 1.0f : s.decay;
+	p.decays = !((e.info >> 60) & 1);
 	p.state = (a.block_base + e.block0) * kStateBlock;
 	p.master = a.master && p.ptype != T_F32 ? a.master + p.state : nullptr;
 	return p;
@@ -300,149 +308,167 @@ __device__ inline Place place_of(const AdamwArgs& a, const TensorEntry& e, const
 
 __device__ inline uint64_t word_of(const Step& s, uint64_t element) { return finalise(s.key + (element >> 3) * kGolden); }
 
-// moments in 32 bits: V elements per lane, U such groups in flight
-template <int V, int U> __device__ inline void chunk32(const AdamwArgs& a, const Step& s, const Place& p, uint64_t first)
-{
-	Raw<V> rg[U], rw[U], rm[U], rv[U];
-	float* const am = static_cast<float*>(a.m) + p.state;
-	float* const av = static_cast<float*>(a.v) + p.state;
-	const int wtype = p.master ? (int) T_F32 : p.ptype;
-	const void* const weights = p.master ? p.master : p.param;
+// A tile with moments in 32 bits: four elements per lane (16 B of every f32 array), U such groups in flight.
+template <int TILE> struct Tile32 {
+	static constexpr int V = 4, U = TILE / kThreads / V;
+	Raw<V> g[U], w[U], m[U], v[U];
+	__device__ static uint64_t at(uint64_t first, int u) { return first + (u * kThreads + threadIdx.x) * V; }
+	__device__ void load(const AdamwArgs& a, const Place& p, uint64_t first)
+	{
 #pragma unroll
-	for (int u = 0; u < U; u++) {
-		const uint64_t i = first + (u * kThreads + threadIdx.x) * V;
-		if (i >= p.n) continue;
-		load<V>(p.grad, i, p.n, p.gtype, rg[u]);
-		load<V>(weights, i, p.n, wtype, rw[u]);
-		fetch<V * 4, 16>(am + i, rm[u].w);
-		fetch<V * 4, 16>(av + i, rv[u].w);
-	}
-#pragma unroll
-	for (int u = 0; u < U; u++) {
-		const uint64_t i = first + (u * kThreads + threadIdx.x) * V;
-		if (i >= p.n) continue;
-		float g[V], w[V], m[V], v[V];
-		widen<V>(rg[u], p.gtype, g);
-		widen<V>(rw[u], wtype, w);
-		uint32_t word = 0;
-		if (s.stochastic) word = (uint32_t) word_of(s, p.state + i) + (uint32_t) (i & 7) * kLaneStep;
-#pragma unroll
-		for (int j = 0; j < V; j++) {
-			m[j] = bits_float(rm[u].w[j]);
-			v[j] = bits_float(rv[u].w[j]);
-			update(s, p.decay, g[j] * s.scale, m[j], v[j], w[j]);
+		for (int u = 0; u < U; u++) {
+			const uint64_t i = at(first, u);
+			if (i >= p.n) continue;
+			sqn::load<V>(p.grad, i, p.n, p.gtype, g[u]);
+			sqn::load<V>(p.weights(), i, p.n, p.wtype(), w[u]);
+			fetch<V * 4, 16>(static_cast<float*>(a.m) + p.state + i, m[u].w);
+			fetch<V * 4, 16>(static_cast<float*>(a.v) + p.state + i, v[u].w);
 		}
-		store32<V>(am, i, p.n, m);
-		store32<V>(av, i, p.n, v);
-		put_weights<V>(s, p.param, i, p.n, p.ptype, p.master, w, word);
 	}
-}
-
-// moments in 8 bits: 16 lanes of eight elements are a block, U such groups in flight
-template <int U> __device__ inline void chunk8(const AdamwArgs& a, const Step& s, const Place& p, uint64_t first)
-{
-	Raw<kLane> rg[U], rw[U];
-	uint32_t cm[U][2], cv[U][2];
-	uint8_t sm[U], sv[U];
-	uint8_t* const am = static_cast<uint8_t*>(a.m) + p.state;
-	uint8_t* const av = static_cast<uint8_t*>(a.v) + p.state;
-	uint8_t* const bm = a.m_scale + p.state / kStateBlock;
-	uint8_t* const bv = a.v_scale + p.state / kStateBlock;
-	const int wtype = p.master ? (int) T_F32 : p.ptype;
-	const void* const weights = p.master ? p.master : p.param;
+	__device__ void work(const AdamwArgs& a, const Step& s, const Place& p, uint64_t first)
+	{
+		const float decay = p.decays ? s.decay : 1.0f;
 #pragma unroll
-	for (int u = 0; u < U; u++) {
-		const uint64_t i = first + (u * kThreads + threadIdx.x) * kLane;
-		if ((i & ~(uint64_t) (kStateBlock - 1)) >= p.n) continue;            // whole blocks of 16 lanes leave together
-		sm[u] = bm[i / kStateBlock];
-		sv[u] = bv[i / kStateBlock];
-		load<kLane>(p.grad, i, p.n, p.gtype, rg[u]);
-		load<kLane>(weights, i, p.n, wtype, rw[u]);
-		fetch<8, 8>(am + i, cm[u]);
-		fetch<8, 8>(av + i, cv[u]);
-	}
+		for (int u = 0; u < U; u++) {
+			const uint64_t i = at(first, u);
+			if (i >= p.n) continue;
+			float fg[V], fw[V], fm[V], fv[V];
+			widen<V>(g[u], p.gtype, fg);
+			widen<V>(w[u], p.wtype(), fw);
+			uint32_t word = 0;
+			if (s.stochastic) word = (uint32_t) word_of(s, p.state + i) + (uint32_t) (i & 7) * kLaneStep;
 #pragma unroll
-	for (int u = 0; u < U; u++) {
-		const uint64_t i = first + (u * kThreads + threadIdx.x) * kLane;
-		if ((i & ~(uint64_t) (kStateBlock - 1)) >= p.n) continue;
-		float g[kLane], w[kLane], m[kLane], v[kLane];
-		widen<kLane>(rg[u], p.gtype, g);
-		widen<kLane>(rw[u], wtype, w);
-		decode<false>(cm[u], scale_float(sm[u]), m);
-		decode<true>(cv[u], scale_float(sv[u]), v);
-		const uint64_t word = word_of(s, p.state + i);
-		// Bits of magnitudes order like the magnitudes, infinity and NaN last.  The first moment's maximum passes over NaN; but
-		// where m is NaN so is v, of the same element.
-		float tm = 0;
-		uint32_t tv = 0;
-#pragma unroll
-		for (int j = 0; j < kLane; j++) {
-			update(s, p.decay, g[j] * s.scale, m[j], v[j], w[j]);
-			tm = fmaxf(tm, fabsf(m[j]));
-			tv = max(tv, float_bits(v[j]) & 0x7fffffffu);
+			for (int j = 0; j < V; j++) {
+				fm[j] = bits_float(m[u].w[j]);
+				fv[j] = bits_float(v[u].w[j]);
+				update(s, decay, fg[j] * s.scale, fm[j], fv[j], fw[j]);
+			}
+			store32<V>(static_cast<float*>(a.m) + p.state, i, p.n, fm);
+			store32<V>(static_cast<float*>(a.v) + p.state, i, p.n, fv);
+			put_weights<V>(s, p.param, i, p.n, p.ptype, p.master, fw, word);
 		}
-		tv = row_reduce(tv, [](uint32_t x, uint32_t y) { return max(x, y); });
-		if (tv >= 0x7f800000u) {
-#pragma unroll
-			for (int j = 0; j < kLane; j++)
-				if (m[j] != m[j]) tm = __builtin_inff();
-		}
-		const uint32_t om = scale_byte(row_reduce(float_bits(tm), [](uint32_t x, uint32_t y) { return max(x, y); }), 7), ov = scale_byte(tv, 14);
-		uint32_t c[2];
-		encode<false>(m, om, (uint32_t) word, c);
-		put<8, 8>(am + i, c);
-		encode<true>(v, ov, (uint32_t) (word >> 32), c);
-		put<8, 8>(av + i, c);
-		if ((threadIdx.x & 15) == 0) { bm[i / kStateBlock] = (uint8_t) om; bv[i / kStateBlock] = (uint8_t) ov; }
-		if (i < p.n) put_weights<kLane>(s, p.param, i, p.n, p.ptype, p.master, w, (uint32_t) word);
 	}
-}
+};
 
-// The step's numbers once for all workgroups: a kernel of one lane in front of the step.  They are a few hundred cycles of f64, and counting
-// the step here needs no workgroup to wait for the others; where every workgroup does it and arrives at one counter, arrivals
-// take 6.5 ns each, one after the other.
-__global__ void k_adamw_begin(const AdamwArgs a)
-{
-	const long long t = a.count[0] + 1;
-	const Step s = step_of(a, t);
-	*a.step = s;
-	if (s.go) a.count[0] = t;
-}
+// A tile with moments in 8 bits: eight elements per lane, so that 16 lanes are a block; U such groups in flight.
+template <int TILE> struct Tile8 {
+	static constexpr int V = kLane, U = TILE / kThreads / V;
+	Raw<V> g[U], w[U];
+	uint32_t m[U][2], v[U][2];
+	uint8_t ms[U], vs[U];
+	__device__ static uint64_t at(uint64_t first, int u) { return first + (u * kThreads + threadIdx.x) * V; }
+	__device__ static bool outside(uint64_t i, uint64_t n) { return (i & ~(uint64_t) (kStateBlock - 1)) >= n; }   // the same for the 16 lanes of a block
+	__device__ void load(const AdamwArgs& a, const Place& p, uint64_t first)
+	{
+#pragma unroll
+		for (int u = 0; u < U; u++) {
+			const uint64_t i = at(first, u);
+			if (outside(i, p.n)) continue;
+			ms[u] = a.m_scale[(p.state + i) / kStateBlock];
+			vs[u] = a.v_scale[(p.state + i) / kStateBlock];
+			sqn::load<V>(p.grad, i, p.n, p.gtype, g[u]);
+			sqn::load<V>(p.weights(), i, p.n, p.wtype(), w[u]);
+			fetch<V, V>(static_cast<uint8_t*>(a.m) + p.state + i, m[u]);
+			fetch<V, V>(static_cast<uint8_t*>(a.v) + p.state + i, v[u]);
+		}
+	}
+	__device__ void work(const AdamwArgs& a, const Step& s, const Place& p, uint64_t first)
+	{
+		const float decay = p.decays ? s.decay : 1.0f;
+		const auto larger = [](uint32_t x, uint32_t y) { return max(x, y); };
+#pragma unroll
+		for (int u = 0; u < U; u++) {
+			const uint64_t i = at(first, u);
+			if (outside(i, p.n)) continue;
+			float fg[V], fw[V], fm[V], fv[V];
+			widen<V>(g[u], p.gtype, fg);
+			widen<V>(w[u], p.wtype(), fw);
+			decode<false>(m[u], scale_float(ms[u]), fm);
+			decode<true>(v[u], scale_float(vs[u]), fv);
+			const uint64_t word = word_of(s, p.state + i);
+			// Bits of magnitudes order like the magnitudes, infinity and NaN last.  The first moment's maximum passes over NaN; but
+			// where m is NaN so is v, of the same element.
+			float tm = 0;
+			uint32_t tv = 0;
+#pragma unroll
+			for (int j = 0; j < V; j++) {
+				update(s, decay, fg[j] * s.scale, fm[j], fv[j], fw[j]);
+				tm = fmaxf(tm, fabsf(fm[j]));
+				tv = max(tv, float_bits(fv[j]) & 0x7fffffffu);
+			}
+			tv = row_reduce(tv, larger);
+			if (tv >= 0x7f800000u) {
+#pragma unroll
+				for (int j = 0; j < V; j++)
+					if (fm[j] != fm[j]) tm = __builtin_inff();
+			}
+			const uint32_t om = scale_byte(row_reduce(float_bits(tm), larger), 7), ov = scale_byte(tv, 14);
+			uint32_t c[2];
+			encode<false>(fm, om, (uint32_t) word, c);
+			put<V, V>(static_cast<uint8_t*>(a.m) + p.state + i, c);
+			encode<true>(fv, ov, (uint32_t) (word >> 32), c);
+			put<V, V>(static_cast<uint8_t*>(a.v) + p.state + i, c);
+			if ((threadIdx.x & 15) == 0) {
+				a.m_scale[(p.state + i) / kStateBlock] = (uint8_t) om;
+				a.v_scale[(p.state + i) / kStateBlock] = (uint8_t) ov;
+			}
+			if (i < p.n) put_weights<V>(s, p.param, i, p.n, p.ptype, p.master, fw, (uint32_t) word);
+		}
+	}
+};
 
-// TILE elements at a time; ALONE: a few workgroups form the step's numbers themselves, and the last to arrive counts the step
-template <int BITS, int TILE, bool ALONE> __global__ __launch_bounds__(kThreads) void k_adamw(const AdamwArgs a)
+// Every workgroup reads the step counter and forms the step's numbers itself, while its first tile is on the way; the last one to
+// arrive, when all others have read it, counts the step.
+template <template <int> class Tile, int TILE, int N> __global__ __launch_bounds__(kThreads) void k_adamw(const Table<AdamwArgs, N> table)
 {
-	const long long t = ALONE ? a.count[0] + 1 : 0;
-	const Step s = ALONE ? step_of(a, t) : *a.step;
-	if (!s.go) return;
-	Cursor<AdamwArgs> cursor(a, blockIdx.x);
-	for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+	const AdamwArgs& a = table.a;
+	Cursor<Table<AdamwArgs, N>> cursor(table, blockIdx.x);
+	Tile<TILE> t;
+	Place p{};
+	uint64_t first = 0;
+	const auto load = [&](uint32_t tile) {
 		const TensorEntry& e = cursor.at(tile);
-		const Place p = place_of(a, e, s);
-		const uint64_t first = (uint64_t) (tile - e.tile0) * TILE;
-		if (BITS == 32) chunk32<4, TILE / kThreads / 4>(a, s, p, first);
-		else chunk8<TILE / kThreads / kLane>(a, s, p, first);
+		p = place_of(a, e);
+		first = (uint64_t) (tile - e.tile0) * TILE;
+		t.load(a, p, first);
+	};
+	uint32_t tile = blockIdx.x;
+	if (tile < a.tiles) load(tile);
+	const long long count = a.count[0] + 1;
+	const Step s = step_of(a, count);
+	if (!s.go) return;
+	while (tile < a.tiles) {
+		t.work(a, s, p, first);
+		tile += gridDim.x;
+		if (tile < a.tiles) load(tile);
 	}
-	if (ALONE && threadIdx.x == 0) {                    // by the last arrival every other workgroup has read the counter
-		unsigned long long* arrived = reinterpret_cast<unsigned long long*>(a.count + 1);
-		if (__hip_atomic_fetch_add(arrived, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
-			__hip_atomic_store(arrived, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-			a.count[0] = t;
-		}
+	if (!a.last || threadIdx.x) return;
+	const uint32_t gate = blockIdx.x % kGates, through = gridDim.x < kGates ? gridDim.x : kGates;
+	uint32_t* arrived = reinterpret_cast<uint32_t*>(a.gates + gate * kGateStride);
+	if (gridDim.x > 1) {
+		if (__hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != (gridDim.x - gate - 1) / kGates) return;
+		__hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+		unsigned long long* all = reinterpret_cast<unsigned long long*>(a.count + 1);
+		if (__hip_atomic_fetch_add(all, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != through - 1) return;
+		__hip_atomic_store(all, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 	}
+	a.count[0] = count;
 }
 
 // ---- the norm ------------------------------------------------------------------------------------------------------------------------
 // Squares are summed in f64: f32 gradients reach 3e38, whose square is past f32, and 1e9 of them add up.  The order is fixed by the sizes
 // alone -- lane, wave, workgroup, then the partial sums by one workgroup -- so that the same gradients give the same bits.
-__device__ inline double block_sum(double x)
+template <int THREADS> __device__ inline double block_sum(double x)
 {
-	__shared__ double wave[kThreads / 64];
+	__shared__ double wave[THREADS / 64];
 #pragma unroll
 	for (int d = 32; d; d >>= 1) x += __shfl_down(x, d);
 	if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = x;
 	__syncthreads();
-	return wave[0] + wave[1] + wave[2] + wave[3];
+	x = wave[0];
+#pragma unroll
+	for (int k = 1; k < THREADS / 64; k++) x += wave[k];
+	return x;
 }
 
 // a norm that is not finite leaves NaN as the coefficient: the step that takes it is rejected
@@ -454,11 +480,12 @@ __device__ inline void verdict(double sum, double grad_scale, double max_norm, f
 	out[1] = !finite ? __builtin_nanf("") : (float) (norm > max_norm ? grad_scale * (max_norm / norm) : grad_scale);
 }
 
-template <int TILE> __global__ __launch_bounds__(kThreads) void k_norm(const NormArgs a)
+template <int TILE, int N> __global__ __launch_bounds__(kThreads) void k_norm(const Table<NormArgs, N> table)
 {
 	constexpr int V = 8, U = TILE / kThreads / V;
+	const NormArgs& a = table.a;
 	double sum = 0;
-	Cursor<NormArgs> cursor(a, blockIdx.x);
+	Cursor<Table<NormArgs, N>> cursor(table, blockIdx.x);
 	for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
 		const TensorEntry& e = cursor.at(tile);
 		const uint64_t n = e.info & kCountMask, first = (uint64_t) (tile - e.tile0) * TILE + threadIdx.x * V;
@@ -476,17 +503,18 @@ template <int TILE> __global__ __launch_bounds__(kThreads) void k_norm(const Nor
 			for (int j = 0; j < V; j++) sum = fma((double) g[j], (double) g[j], sum);
 		}
 	}
-	sum = block_sum(sum);
+	sum = block_sum<kThreads>(sum);
 	if (threadIdx.x) return;
 	if (a.out) verdict(sum, a.grad_scale, a.max_norm, a.out);
 	else a.part[blockIdx.x] = sum;
 }
 
-__global__ __launch_bounds__(kThreads) void k_norm_sum(double* part, int count, double grad_scale, double max_norm, float* out)
+constexpr int kSumThreads = 1024;
+__global__ __launch_bounds__(kSumThreads) void k_norm_sum(double* part, int count, double grad_scale, double max_norm, float* out)
 {
 	double sum = 0;
-	for (int i = threadIdx.x; i < count; i += kThreads) sum += part[1 + i];
-	sum = block_sum(sum);
+	for (int i = threadIdx.x; i < count; i += kSumThreads) sum += part[1 + i];
+	sum = block_sum<kSumThreads>(sum);
 	if (threadIdx.x) return;
 	part[0] = sum;
 	if (out) verdict(sum, grad_scale, max_norm, out);
@@ -496,25 +524,35 @@ __global__ void k_norm_verdict(const double* sum, double grad_scale, double max_
 
 }  // namespace
 
-void launch_adamw_begin(hipStream_t st, const AdamwArgs& a) { k_adamw_begin<<<1, 1, 0, st>>>(a); }
-void launch_adamw(hipStream_t st, int bits, int tile, int grid, const AdamwArgs& a)
+// a short list travels in a short table
+template <class Args> static Table<Args, kFewEntries> few(const Table<Args, kEntries>& t)
 {
-	if (bits == 8) {
-		if (a.step) tile == kTileSmall ? k_adamw<8, kTileSmall, false><<<grid, kThreads, 0, st>>>(a) : k_adamw<8, kTile8, false><<<grid, kThreads, 0, st>>>(a);
-		else k_adamw<8, kTileSmall, true><<<grid, kThreads, 0, st>>>(a);
-	} else {
-		if (a.step) tile == kTileSmall ? k_adamw<32, kTileSmall, false><<<grid, kThreads, 0, st>>>(a) : k_adamw<32, kTile32, false><<<grid, kThreads, 0, st>>>(a);
-		else k_adamw<32, kTileSmall, true><<<grid, kThreads, 0, st>>>(a);
-	}
+	Table<Args, kFewEntries> f;
+	f.a = t.a;
+	for (int k = 0; k < t.a.entries; k++) f.entry[k] = t.entry[k];
+	return f;
 }
-void launch_norm(hipStream_t st, int tile, int grid, const NormArgs& a)
+
+template <template <int> class Tile, int LARGE> static void launch_tiles(hipStream_t st, int tile, int grid, const Table<AdamwArgs, kEntries>& t)
 {
-	if (tile == kTileSmall) k_norm<kTileSmall><<<grid, kThreads, 0, st>>>(a);
-	else k_norm<kTile8><<<grid, kThreads, 0, st>>>(a);
+	if (tile != kTileSmall) k_adamw<Tile, LARGE, kEntries><<<grid, kThreads, 0, st>>>(t);
+	else if (t.a.entries > kFewEntries) k_adamw<Tile, kTileSmall, kEntries><<<grid, kThreads, 0, st>>>(t);
+	else k_adamw<Tile, kTileSmall, kFewEntries><<<grid, kThreads, 0, st>>>(few(t));
+}
+void launch_adamw(hipStream_t st, int bits, int tile, int grid, const Table<AdamwArgs, kEntries>& t)
+{
+	if (bits == 8) launch_tiles<Tile8, kTile8>(st, tile, grid, t);
+	else launch_tiles<Tile32, kTile32>(st, tile, grid, t);
+}
+void launch_norm(hipStream_t st, int tile, int grid, const Table<NormArgs, kEntries>& t)
+{
+	if (tile != kTileSmall) k_norm<kTile8, kEntries><<<grid, kThreads, 0, st>>>(t);
+	else if (t.a.entries > kFewEntries) k_norm<kTileSmall, kEntries><<<grid, kThreads, 0, st>>>(t);
+	else k_norm<kTileSmall, kFewEntries><<<grid, kThreads, 0, st>>>(few(t));
 }
 void launch_norm_sum(hipStream_t st, double* part, int count, double grad_scale, double max_norm, float* out)
 {
-	k_norm_sum<<<1, kThreads, 0, st>>>(part, count, grad_scale, max_norm, out);
+	k_norm_sum<<<1, kSumThreads, 0, st>>>(part, count, grad_scale, max_norm, out);
 }
 void launch_norm_verdict(hipStream_t st, const double* sum, double grad_scale, double max_norm, float* out)
 {

@@ -13,6 +13,7 @@ constexpr int kTileSmall = 2048;     // elements a workgroup of 256 threads take
 constexpr int kTile32 = 4096;        // and of many, with moments in 32 bits,
 constexpr int kTile8 = 8192;         // in 8 bits, and for the norm
 constexpr int kEntries = 112;        // tensors per launch: the table travels in the kernel's arguments (32 B each, 4 KB in all)
+constexpr int kFewEntries = 12;      // ... of a short list, whose launch then costs less
 
 enum TensorType { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
 inline size_t type_size(int t) { return t == T_F32 ? 4 : 2; }
@@ -37,47 +38,43 @@ struct LaunchShape {
 	int grid;                    // most workgroups
 };
 
-// What is the same for every element of a step (tensors.hip: step_of)
-struct Step {
-	float scale, b1, b2, a1, a2, decay, rate, root, eps;
-	int stochastic, careful, go;                         // go = 0: rejected
-	uint64_t key;
-};
-constexpr size_t kStepBytes = 64;
-static_assert(sizeof(Step) <= kStepBytes, "the caller's work area");
+// Workgroups arrive at one of these counters, the last of each at count[1]: arrivals at one address take 6.5 ns each, one after the other.
+constexpr int kGates = 16, kGateStride = 256;            // bytes
 
 struct AdamwArgs {
-	TensorEntry entry[kEntries];
 	int entries;                 // of the table that are in use
 	uint32_t tiles;
 	uint64_t block_base;
 	float* master;               // f32 weights of the 16-bit tensors, or NULL
 	void *m, *v;                 // f32[state] or codes [state]
 	uint8_t *m_scale, *v_scale;  // [state / kStateBlock], 8-bit moments only
-	long long* count;            // [0] steps taken, [1] workgroups that have arrived (zero between steps)
-	Step* step;                  // where launch_adamw_begin left the step's numbers; NULL: every workgroup forms them
+	long long* count;            // [0] steps taken, [1] arrivals (zero between steps)
+	char* gates;                 // kGates counters (zero between steps)
 	const float* grad_scale;     // what every gradient is multiplied with; NULL = 1
 	const float* step_size_dev;  // NULL: step_size
 	double step_size, beta1, beta2, weight_decay;
 	float eps;
 	uint64_t seed;
+	int last;                    // the launch that counts the step
 	int stochastic;              // bf16 parameters without f32 weights beside them are rounded stochastically
 };
-static_assert(sizeof(AdamwArgs) <= 4096, "kernel arguments");
 
 struct NormArgs {
-	TensorEntry entry[kEntries]; // param unused
 	int entries;
 	uint32_t tiles;
 	double* part;                // one partial sum of squares per workgroup of this launch
 	double grad_scale, max_norm;
 	float* out;                  // not NULL: this workgroup, the only one, finishes
 };
-static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
 
-void launch_adamw_begin(hipStream_t st, const AdamwArgs& a);      // the step's numbers -> a.step, and the step is counted
-void launch_adamw(hipStream_t st, int bits, int tile, int grid, const AdamwArgs& a);
-void launch_norm(hipStream_t st, int tile, int grid, const NormArgs& a);
+template <class Args, int N> struct Table {
+	Args a;
+	TensorEntry entry[N];
+};
+static_assert(sizeof(Table<AdamwArgs, kEntries>) <= 4096, "kernel arguments");
+
+void launch_adamw(hipStream_t st, int bits, int tile, int grid, const Table<AdamwArgs, kEntries>& t);
+void launch_norm(hipStream_t st, int tile, int grid, const Table<NormArgs, kEntries>& t);      // TensorEntry::param unused
 // part[0] <- the sum of part[1 .. count] (in a fixed order); with `out` also the verdict
 void launch_norm_sum(hipStream_t st, double* part, int count, double grad_scale, double max_norm, float* out);
 // the verdict of a sum of squares that is final: out[0] the norm, out[1] the coefficient

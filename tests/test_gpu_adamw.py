@@ -539,7 +539,7 @@ def test_refusals_of_the_c_entries(capfd):
     n = 1000
     p = torch.zeros(n, device="cuda")
     st = [torch.zeros(1024, device="cuda") for _ in range(3)]
-    count, work = torch.zeros(2, dtype=torch.int64, device="cuda"), torch.zeros(8, dtype=torch.int64, device="cuda")
+    count, work = torch.zeros(2, dtype=torch.int64, device="cuda"), torch.zeros(512, dtype=torch.int64, device="cuda")
     one = lambda ptr, size=n, type=0: lib.stochqn_hip_tensors_create(1, (C.c_void_p * 1)(ptr), (C.c_size_t * 1)(size), (C.c_int * 1)(type))
     hostmem = np.zeros(n, dtype=np.float32)
     for bad in (dict(ptr=hostmem.ctypes.data), dict(ptr=None), dict(ptr=p.data_ptr() + 2), dict(ptr=p.data_ptr(), size=2 ** 40), dict(ptr=p.data_ptr(), size=2 ** 42),
