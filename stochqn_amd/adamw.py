@@ -192,6 +192,7 @@ class AdamW_free:
         self._handle = self._lib.stochqn_hip_adamw_create(self.params._handle, C.byref(setup))
         if not self._handle:
             raise ValueError("the library refused the optimizer (its reason is on stderr).")
+        self._versioned = [t for t in self.tensors if not t.is_inference()]
         self.gradient = None
         self._own_list = False          # `gradient` was made here, so its tensors may be exchanged here
 
@@ -227,6 +228,7 @@ class AdamW_free:
         scale = _scalar(grad_scale, dev, "grad_scale")
         if self._lib.stochqn_hip_adamw_step(self._handle, self.gradient._handle, step_size, step_dev, scale, _stream(dev.index)) != 0:
             raise RuntimeError("stochqn_hip_adamw_step failed (its reason is on stderr).")
+        torch.autograd.graph.increment_version(self._versioned)          # a graph that saved the old weights cannot be run backward any more
 
     def moments(self, i):
         """The two moments of tensor i as float32, in its shape (copies for 8-bit moments, views otherwise)."""

@@ -161,6 +161,9 @@ void set_items(std::vector<Item>& items, int& device, void* const ptr[])
 	device = on;
 }
 
+// Tiles of a launch with several tensors: their blocks are counted in 32 bits (64 to the largest tile).
+constexpr uint64_t kMostTiles = 1 << 25;
+
 // The tables of a list, one launch after the other: fill(i, entry) for every tensor with elements, fire(base block, entries, tiles) for every
 // table that is full or the last.
 template <class Fill, class Fire> void for_launches(const std::vector<Item>& items, int tile, TensorEntry* entry, Fill&& fill, Fire&& fire)
@@ -170,7 +173,7 @@ template <class Fill, class Fire> void for_launches(const std::vector<Item>& ite
 	for (size_t i = 0; i < items.size(); i++) {
 		if (!items[i].n) continue;
 		const uint64_t mine = tiles_of(items[i].n, tile);
-		if (used == kEntries || (used && tiles + mine > 0x7fffffffu)) {
+		if (used == kEntries || (used && tiles + mine > kMostTiles)) {
 			fire(used, (uint32_t) tiles, false);
 			used = 0;
 			tiles = 0;
@@ -255,6 +258,7 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors* t, double grad_scale, double m
 		check_memory(work, stochqn_hip_tensors_norm_work(t) * sizeof(double), device, "work");
 		OnDevice on(device);
 		hipStream_t st = check_stream(hip_stream, device);
+		(void) hipGetLastError();                                  // somebody else's: only what the launches below leave counts
 		const bool reduced = comm_nranks() > 1;
 		Table<NormArgs, kEntries> table;
 		NormArgs& a = table.a;
@@ -365,6 +369,7 @@ int stochqn_hip_adamw_step(stochqn_hip_adamw* o, stochqn_hip_tensors* grads, dou
 		check_scalar(grad_scale, o->device, "grad_scale");
 		OnDevice on(o->device);
 		hipStream_t st = check_stream(hip_stream, o->device);
+		(void) hipGetLastError();
 		const stochqn_hip_adamw_setup& s = o->s;
 		Table<AdamwArgs, kEntries> table;
 		AdamwArgs& a = table.a;

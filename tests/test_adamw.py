@@ -82,3 +82,14 @@ def test_the_words_are_uniform():
     assert abs(np.corrcoef(low.astype(float), again.astype(float))[0, 1]) < 6 / np.sqrt(low.size)
     part, _ = ref.words(1000, 77, 12345, 7)
     assert (part == low[1000:1077]).all()
+
+
+@pytest.mark.parametrize("which", ["asan", "tsan"])
+def test_the_host_side_under_sanitizers(which):
+    """What tensors.cpp hands to the kernels (every element of every tensor in one tile of one launch) and what it refuses, every HIP call failing
+    in turn; threads that step, rebind and take the norm of one list at once."""
+    here = os.path.join(ROOT, "tests", "hostsim")
+    subprocess.check_call(["make", "-C", here, "build/tensors_" + which], stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
+    for args in ([], ["threads"]) if which == "asan" else (["threads"],):
+        run = subprocess.run([os.path.join(here, "build", "tensors_" + which)] + args, capture_output=True, text=True, timeout=300)
+        assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr[-3000:]

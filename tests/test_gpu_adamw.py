@@ -230,6 +230,39 @@ def test_eight_bit_blocks_with_nothing_tiny_huge_and_not_finite():
     assert model.params[0][7 * 128:9 * 128].isnan().all()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tiny_gradients_beside_a_tiny_eps(bits):
+    """Second moments among the subnormals of 32 bits, eps below their roots: with beta1 = 0, beta2 = 0.5 the first step is lr * g / (|g| + eps).
+
+    v = g^2 / 2 carries three roundings of at most half of 2^-149 each there (square, product, sum), or 6 u relative: its root half of that
+    relative, to first order, 0.6 of it up to a tenth; the other roundings of the update are 10 u (2 root, 1 q, 1 sum, 1 eps, 3 quotient, 1 r,
+    1 last sum)."""
+    g = np.array([s * m * 10.0 ** -e for e in range(13, 22) for m in (1.0, 1.7, 3.3, 7.1) for s in (1, -1)], dtype=np.float32)
+    w = torch.zeros(g.size, device="cuda")
+    opt = stochqn().AdamW_free([w], beta1=0.0, beta2=0.5, eps=1e-30, weight_decay=0.0, state_bits=bits)
+    opt.update_gradient([torch.as_tensor(g).cuda()])
+    opt.run_optimizer(1.0)
+    g = g.astype(np.float64)
+    v = g * g / 2
+    off = np.maximum(6 * 2.0 ** -24, 3 * 2.0 ** -150 / v)
+    sure = off < 0.1
+    assert sure.sum() > 50 and (v[sure] < 2.0 ** -126).sum() >= 10
+    want = -g / (np.abs(g) + 1e-30)
+    assert (np.abs(host(w) - want)[sure] <= ((0.6 * off + 10 * 2.0 ** -24) * np.abs(want))[sure]).all()
+
+
+def test_autograd_knows_that_the_weights_were_written():
+    w = torch.randn(100, device="cuda", requires_grad=True)
+    x = torch.ones(100, device="cuda")
+    opt = stochqn().AdamW_free([w])
+    loss = (w * w * x).sum()
+    loss.backward(retain_graph=True)
+    opt.update_gradient([w.grad])
+    opt.run_optimizer(LR)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()                                     # the saved weights are not the ones that the loss was computed from
+
+
 def test_stochastic_rounding_keeps_the_mean_and_moves_what_nearest_leaves():
     """v from a constant gradient: after k steps E v = (1 - b2^k) g^2.  One step moves v by at most a hundredth of a step of e5m2 at the end, so that
     rounding to nearest would stop; the mean over 2^16 elements has to be within five standard errors, measured from the elements."""
