@@ -205,7 +205,7 @@ class AdamW_free:
             self.gradient, self._own_list = gradient, False
             return
         gradient = list(gradient)
-        if self._own_list and [t.dtype for t in gradient] == self.gradient.dtypes:
+        if self._own_list and [getattr(t, "dtype", None) for t in gradient] == self.gradient.dtypes:
             self.gradient.rebind(gradient)
             return
         new = TensorList(gradient)

@@ -230,6 +230,21 @@ def test_eight_bit_blocks_with_nothing_tiny_huge_and_not_finite():
     assert model.params[0][7 * 128:9 * 128].isnan().all()
 
 
+def test_eight_bit_codes_of_subnormal_moments():
+    """Blocks whose moments lie among the subnormals of 32 bits, where the scale's exponent has reached its least: the codes are still the ones of
+    the emulation, for each moment at each size."""
+    n = 128 * 40
+    model = Model([n], F32, F32, seed=2)
+    base = np.random.default_rng(7).standard_normal(n).reshape(40, 128)
+    for scale in (10.0 ** -np.linspace(14, 23, 40), 10.0 ** -np.linspace(33, 44, 40)):
+        opt = stochqn().AdamW_free(model.params, state_bits=8, seed=11)
+        opt.update_gradient(model.grads)
+        for _ in range(3):
+            model.grads[0].copy_(torch.as_tensor((base * scale[:, None]).astype(np.float32).reshape(-1)))
+            check_step(model, opt)
+            base = np.roll(base, 1, axis=1)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_tiny_gradients_beside_a_tiny_eps(bits):
     """Second moments among the subnormals of 32 bits, eps below their roots: with beta1 = 0, beta2 = 0.5 the first step is lr * g / (|g| + eps).
@@ -544,6 +559,11 @@ def test_refusals():
     for bad in ([torch.zeros(299, device="cuda")], [torch.zeros(300)], [torch.zeros(300, device="cuda")] * 2, [torch.zeros(600, device="cuda")[::2]]):
         with pytest.raises(ValueError):
             opt.update_gradient(bad)
+    with pytest.raises(ValueError):
+        opt.update_gradient([None])                         # a parameter that has no gradient yet
+    opt.update_gradient([torch.zeros(300, device="cuda")])
+    with pytest.raises(ValueError):
+        opt.update_gradient([None])
     opt.update_gradient([p])                                # the gradient is the weights themselves
     with pytest.raises(RuntimeError):
         opt.run_optimizer(LR)
