@@ -18,8 +18,8 @@ using namespace sqn;
 
 namespace {
 
-// Most workgroups per compute unit (measured at 1.28e9 elements): 32-bit moments 4, 8 and 16 alike; 8-bit moments 2.53 ms with 8, 2.46 with 16,
-// 2.41 with 32; the norm 466 us with 4, 380 with 8, 384 with 16.
+// Most workgroups per compute unit.  Measured at 1.28e9 elements: 32-bit moments 6.58 - 6.66 ms from 4 to 32; 8-bit moments 2.53 ms with 8, 2.47 with
+// 16, 2.44 with 32, 2.46 with 64; the norm 466 us with 4, 377 with 8, 379 with 16.
 constexpr int kPerUnit32 = 8, kPerUnit8 = 32, kPerUnitNorm = 8;
 
 struct Range { const char* at; size_t bytes; };                              // of device memory
@@ -68,9 +68,9 @@ void check_aligned(const void* p, size_t to, const char* what)
 
 uint64_t tiles_of(size_t n, int tile) { return (n + tile - 1) / tile; }
 
-// Large tiles keep more loads of a lane in flight; a list with fewer than `few` of them for each compute unit is cut into small ones.  Measured at
-// 7.7e6 elements: the step with 8-bit moments 21.1 us small, 24.2 large (3.7 a unit), with 32-bit moments 44.8 and 46.3 (7.4 a unit); the
-// norm, whose partial sums have to be added up, 12.6 and 11.0.
+// Large tiles keep more loads of a lane in flight; a list with fewer than `few` of them for each compute unit is cut into small ones, so that
+// every unit has work.  Measured at 7.7e6 elements: the step with 8-bit moments 22.6 us small, 24.1 large (3.7 large tiles a unit), with
+// 32-bit moments 42.3 and 44.8 (7.4 a unit); the norm, whose partial sums have to be added up, 12.6 and 9.4.
 constexpr int kFewStep = 8, kFewNorm = 2;
 LaunchShape shape_of(const std::vector<Item>& items, int units, int large, int few, int per_unit)
 {
