@@ -307,8 +307,9 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors *tensors, double grad_scale, do
  *   work              4096 bytes, aligned to 8, zero: arrivals as well
  * m, v, master aligned to 16 bytes.  eps >= 2^-126.  No two arrays that the step writes may overlap, nor a gradient with one.
  * step:  grads: as many tensors, of the same sizes, f32 / bf16 / f16 each; step_size_dev (nullable): a float on the device in place of
- * step_size (schedules in a captured graph); grad_scale (nullable = 1): a float on the device, out + 1 of the norm.  Not finite: the step
- * is rejected, nothing is written and nothing counted -- the guard of take_step, left on the device.  Returns 0 or -1000. */
+ * step_size (schedules in a captured graph); grad_scale (nullable = 1): a float on the device, out + 1 of the norm.  If either
+ * is not finite the step is rejected: nothing is written and nothing counted -- the guard of take_step, left on the device.  Returns 0 or
+ * -1000. */
 typedef struct stochqn_hip_adamw_setup {
 	double beta1, beta2, eps, weight_decay;
 	int state_bits, stochastic;

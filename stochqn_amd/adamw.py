@@ -78,6 +78,8 @@ class TensorList:
             raise ValueError("no tensors.")
         if not all(getattr(t, "dtype", None) in types for t in self.tensors):
             raise ValueError("tensors have to be float32, bfloat16 or float16.")
+        if not self.tensors[0].is_cuda:
+            raise ValueError("tensors have to be on one GPU.")
         n = len(self.tensors)
         self.device = self.tensors[0].device
         self._index = self.tensors[0].get_device()
@@ -96,7 +98,7 @@ class TensorList:
         for t, n, dtype in zip(tensors, self.sizes, self.dtypes):
             if t.numel() != n or t.dtype != dtype:
                 raise ValueError("the tensors have other sizes or types than the list's.")
-            if t.get_device() != self._index or not t.is_cuda:
+            if t.get_device() != self._index:
                 raise ValueError("tensors have to be on one GPU.")
             if not t.is_contiguous():
                 raise ValueError("tensors have to be contiguous.")
@@ -117,6 +119,9 @@ class TensorList:
 
     def __len__(self):
         return len(self.tensors)
+
+    def __getstate__(self):
+        raise TypeError("a TensorList holds a handle of the library: make a new one of the tensors")
 
     def norm(self, max_norm=None, grad_scale=1.0, out=None):
         """A float32 tensor of two elements on the device: the norm over all tensors times `grad_scale` (1 / loss scale), and the factor
@@ -192,6 +197,11 @@ class AdamW_free:
         self._handle = self._lib.stochqn_hip_adamw_create(self.params._handle, C.byref(setup))
         if not self._handle:
             raise ValueError("the library refused the optimizer (its reason is on stderr).")
+        # The state is complete when the object is there, whichever stream the steps will use ...
+        self._on = _stream(dev.index)
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(dev).synchronize()
+        self._streams = {self._on}
         self._versioned = [t for t in self.tensors if not t.is_inference()]
         self.gradient = None
         self._own_list = False          # `gradient` was made here, so its tensors may be exchanged here
@@ -215,8 +225,8 @@ class AdamW_free:
 
     def run_optimizer(self, step_size, grad_scale=None):
         """One step.  step_size: a number, or a float32 tensor of one element on the device (schedules in a captured graph).  grad_scale: None,
-        or such a tensor that every gradient is multiplied with (`TensorList.norm(...)[1:]`); if it is not finite the step is rejected:
-        no weight, no moment and no count changes."""
+        or such a tensor that every gradient is multiplied with (`TensorList.norm(...)[1:]`).  If either is not finite the step is
+        rejected: no weight, no moment and no count changes."""
         if self.gradient is None:
             raise ValueError("no gradient: call update_gradient first.")
         dev = self.params.device
@@ -226,9 +236,24 @@ class AdamW_free:
         elif not math.isfinite(step_size):
             raise ValueError("'step_size' is not finite.")
         scale = _scalar(grad_scale, dev, "grad_scale")
-        if self._lib.stochqn_hip_adamw_step(self._handle, self.gradient._handle, step_size, step_dev, scale, _stream(dev.index)) != 0:
+        stream = _stream(dev.index)
+        if stream != self._on:
+            self._used_on(stream)
+        if self._lib.stochqn_hip_adamw_step(self._handle, self.gradient._handle, step_size, step_dev, scale, stream) != 0:
             raise RuntimeError("stochqn_hip_adamw_step failed (its reason is on stderr).")
         torch.autograd.graph.increment_version(self._versioned)          # a graph that saved the old weights cannot be run backward any more
+
+    def _used_on(self, stream):
+        """... and its memory is not given to others before the work of those streams is done."""
+        self._on = stream
+        if stream not in self._streams and not torch.cuda.is_current_stream_capturing():
+            self._streams.add(stream)
+            for t in (self.m, self.v, self.m_scale, self.v_scale, self.master, self.count, self._work):
+                if t is not None:
+                    t.record_stream(torch.cuda.current_stream(self.params.device))
+
+    def __getstate__(self):
+        raise TypeError("an AdamW_free holds a handle of the library: carry its state_dict() instead")
 
     def moments(self, i):
         """The two moments of tensor i as float32, in its shape (copies for 8-bit moments, views otherwise)."""

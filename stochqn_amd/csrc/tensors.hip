@@ -171,9 +171,10 @@ struct Step {
 __device__ inline Step step_of(const AdamwArgs& a, long long t)
 {
 	Step s{};
-	// a scale that is not finite: the step is rejected as a whole, nothing changes and nothing is counted
+	// a scale or a step size that is not finite: the step is rejected as a whole, nothing changes and nothing is counted
+	const double lr = a.step_size_dev ? (double) *a.step_size_dev : a.step_size;
 	s.scale = a.grad_scale ? *a.grad_scale : 1.0f;
-	s.go = fabsf(s.scale) <= 3.402823466e38f;
+	s.go = __builtin_isfinite(s.scale) && __builtin_isfinite(lr);
 	if (!s.go) return s;
 	double p1 = 1, p2 = 1, q1 = a.beta1, q2 = a.beta2;       // b^t by squaring, in f64: 1 - b2^t loses ten bits at t = 1
 	for (unsigned long long k = (unsigned long long) t; k; k >>= 1) {
@@ -181,7 +182,6 @@ __device__ inline Step step_of(const AdamwArgs& a, long long t)
 		q1 *= q1;
 		q2 *= q2;
 	}
-	const double lr = a.step_size_dev ? (double) *a.step_size_dev : a.step_size;
 	s.b1 = (float) a.beta1;
 	s.b2 = (float) a.beta2;
 	s.a1 = (float) (1 - a.beta1);

@@ -190,6 +190,10 @@ def test_a_scale_from_the_device_and_a_rejected_step(bits):
         opt.run_optimizer(LR, grad_scale=scale)
         assert all((t.view(torch.uint8) == w).all() for t, w in zip(kept, was)), bad
     scale.fill_(1.0)
+    for bad in (math.nan, math.inf):
+        rate.fill_(bad)
+        opt.run_optimizer(rate, grad_scale=scale)
+        assert all((t.view(torch.uint8) == w).all() for t, w in zip(kept, was)), bad
     check_step(model, opt, grad_scale=scale)
 
 
@@ -433,6 +437,42 @@ def test_on_another_stream_and_from_two_threads():
             clip = opts[1][k].gradient.norm(max_norm=0.5)
             opts[1][k].run_optimizer(LR, grad_scale=clip[1:])
         assert all((p == q).all() for p, q in zip(models[k].params, twins[k].params))
+
+
+def test_the_state_outlives_the_work_of_every_stream_that_used_it():
+    """An object made on one stream, used on another and dropped at once: its memory must not come back while the step is still running.  The second
+    stream is kept busy in front of the step; what is allocated and filled after the drop is then looked at."""
+    sq = stochqn()
+    n = 1 << 20
+    w, g = torch.zeros(n, device="cuda"), torch.ones(n, device="cuda")
+    big = torch.randn(4096, 4096, device="cuda")
+    opt = sq.AdamW_free([w])
+    opt.update_gradient([g])
+    size = opt.m.numel()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(200):
+            big = big @ big
+            big = big / big.abs().max()
+        opt.run_optimizer(LR)
+    del opt
+    fresh = [torch.full((size,), 7.0, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all((f == 7).all() for f in fresh)
+    want = -LR * 1.0 / (1.0 + 1e-8)
+    assert (w.double() - want).abs().max() <= 13 * 2.0 ** -24 * LR
+
+
+def test_copies_are_refused():
+    import copy
+    import pickle
+    sq = stochqn()
+    opt = sq.AdamW_free([torch.zeros(4, device="cuda")])
+    for thing in (opt, opt.params):
+        for how in (copy.copy, copy.deepcopy, pickle.dumps):
+            with pytest.raises(TypeError):
+                how(thing)
 
 
 def test_rebinding_gradients_and_state_dicts():
