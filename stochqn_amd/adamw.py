@@ -50,8 +50,12 @@ def _types():
 
 
 def _stream(index):
-    """The current torch stream of a device, as the address that the library takes (torch.cuda.current_stream makes an object: 2 us)."""
-    return torch._C._cuda_getCurrentRawStream(index)
+    """The current torch stream of a device, as the address that the library takes."""
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same without the 2 us that an object for the stream takes
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream)
 
 
 def _scalar(t, device, what):
