@@ -171,7 +171,8 @@ class AdamW_free:
         self.params = params if isinstance(params, TensorList) else TensorList(params)
         self.tensors = list(self.params.tensors)        # what the steps write, whatever the list is rebound to later
         assert not (stochastic and torch.float16 in self.params.dtypes)
-        assert decay is None or len(decay) == len(self.params)
+        if decay is not None and len(decay) != len(self.params):
+            raise ValueError("'decay' has to have one truth value per tensor.")
         self.beta1, self.beta2, self.eps, self.weight_decay = float(beta1), float(beta2), float(eps), float(weight_decay)
         self.state_bits, self.stochastic, self.seed = int(state_bits), bool(stochastic), int(seed) % 2 ** 64
         self.decay = None if decay is None else [bool(d) for d in decay]

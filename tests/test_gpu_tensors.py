@@ -587,12 +587,15 @@ def test_refusals():
     for bad in ([p, p], [p[:200], p[199:]]):                # the same weights twice
         with pytest.raises(ValueError):
             sq.AdamW_free(bad)
-    for kw in (dict(beta1=1.0), dict(beta2=-0.1), dict(eps=0.0), dict(eps=1e-39), dict(state_bits=16), dict(master=True, stochastic=True), dict(decay=[True, False]),
+    for kw in (dict(beta1=1.0), dict(beta2=-0.1), dict(eps=0.0), dict(eps=1e-39), dict(state_bits=16), dict(master=True, stochastic=True),
                dict(weight_decay=math.nan)):
         with pytest.raises(AssertionError):
             sq.AdamW_free([p], **kw)
     with pytest.raises(AssertionError):
         sq.AdamW_free([p.half()], stochastic=True)
+    for bad in ([], [True, False]):
+        with pytest.raises(ValueError):
+            sq.AdamW_free([p], decay=bad)
     opt = sq.AdamW_free([p])
     with pytest.raises(ValueError):
         opt.run_optimizer(LR)                               # no gradient
