@@ -9,18 +9,22 @@
 #include <cfloat>
 #include <cmath>
 #include <cstdio>
+#include <initializer_list>
+#include <memory>
 #include <mutex>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 using namespace sqn;
 
 namespace {
 
-// Most workgroups per compute unit.  Measured at 1.28e9 elements: 32-bit moments 6.58 - 6.66 ms from 4 to 32; 8-bit moments 2.53 ms with 8, 2.47 with
+// Most workgroups per compute unit.  Measured at 1.28e9 elements: 32-bit moments 6.51 ms with 8, 6.50 with 16 (at 7.7e6 elements
+// 43.3 and 40.3 us); 8-bit moments 2.53 ms with 8, 2.47 with
 // 16, 2.44 with 32, 2.46 with 64; the norm 466 us with 4, 377 with 8, 379 with 16.
-constexpr int kPerUnit32 = 8, kPerUnit8 = 32, kPerUnitNorm = 8;
+constexpr int kPerUnit32 = 16, kPerUnit8 = 32, kPerUnitNorm = 8;
 
 struct Range { const char* at; size_t bytes; };                              // of device memory
 bool before(const Range& a, const Range& b) { return a.at < b.at; }
@@ -68,15 +72,17 @@ void check_aligned(const void* p, size_t to, const char* what)
 
 uint64_t tiles_of(size_t n, int tile) { return (n + tile - 1) / tile; }
 
-// Large tiles keep more loads of a lane in flight; a list with fewer than `few` of them for each compute unit is cut into small ones, so that
-// every unit has work.  Measured at 7.7e6 elements: the step with 8-bit moments 22.6 us small, 24.1 large (3.7 large tiles a unit), with
-// 32-bit moments 42.3 and 44.8 (7.4 a unit); the norm, whose partial sums have to be added up, 12.6 and 9.4.
-constexpr int kFewStep = 8, kFewNorm = 2;
-LaunchShape shape_of(const std::vector<Item>& items, int units, int large, int few, int per_unit)
+// Large tiles keep more loads of a lane in flight; a list with fewer than `few` of them for each compute unit is cut into smaller ones, so that
+// every unit has work.  Measured at 7.7e6 elements: the step with 8-bit moments 21.7 us small, 24.1 large (3.7 large tiles a unit), with 32-bit
+// moments 40.3 and 44.8 (7.4 a unit); the norm 12.6 us with tiles of 2048, 9.3 with 8192 (3.7 a unit), 10.3 with 16384 (1.8).
+LaunchShape shape_of(const std::vector<Item>& items, int units, int per_unit, std::initializer_list<std::pair<int, int>> tile_and_few)
 {
-	uint64_t tiles = 0;
-	for (const Item& it : items) tiles += tiles_of(it.n, large);
-	return {tiles < few * (uint64_t) units ? kTileSmall : large, units * per_unit};
+	for (const auto& [tile, few] : tile_and_few) {
+		uint64_t tiles = 0;
+		for (const Item& it : items) tiles += tiles_of(it.n, tile);
+		if (tiles >= few * (uint64_t) units) return {tile, units * per_unit};
+	}
+	return {kTileSmall, units * per_unit};
 }
 
 size_t blocks_of(size_t n) { return (n + kStateBlock - 1) / kStateBlock; }
@@ -204,7 +210,7 @@ stochqn_hip_tensors* stochqn_hip_tensors_create(int count, void* const ptr[], co
 		set_items(t->items, t->device, ptr);
 		if (t->device < 0 && hipGetDevice(&t->device) != hipSuccess) refuse("no current device");
 		t->units = units_of(t->device);
-		t->norm = shape_of(t->items, t->units, kTile8, kFewNorm, kPerUnitNorm);
+		t->norm = shape_of(t->items, t->units, kPerUnitNorm, {{kTileNorm, 4}, {kTileNormMid, 2}});
 		t->version = ++g_versions;
 		return t.release();
 	});
@@ -306,7 +312,7 @@ stochqn_hip_adamw* stochqn_hip_adamw_create(stochqn_hip_tensors* params, const s
 		std::lock_guard<std::mutex> lk(params->mu);
 		o->items = params->items;
 		o->device = params->device;
-		o->shape = s.state_bits == 8 ? shape_of(o->items, params->units, kTile8, kFewStep, kPerUnit8) : shape_of(o->items, params->units, kTile32, kFewStep, kPerUnit32);
+		o->shape = s.state_bits == 8 ? shape_of(o->items, params->units, kPerUnit8, {{kTile8, 8}}) : shape_of(o->items, params->units, kPerUnit32, {{kTile32, 8}});
 		o->s = s;
 		size_t blocks = 0;
 		for (size_t i = 0; i < o->items.size(); i++) {

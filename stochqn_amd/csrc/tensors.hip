@@ -4,11 +4,11 @@
 //   g <- grad_scale * g;   m <- b1 m + (1 - b1) g;   v <- b2 v + (1 - b2) g^2
 //   w <- w (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // Every array is read once and written once; nothing is reused, so HBM bounds the step: 28 B per element with f32 weights and
-// moments, 10 B with bf16 weights and 8-bit moments.  Reached (MI355X): 1e8 f32 elements 487 us = 5.75 TB/s, where four read and three
-// write streams without arithmetic reach 5.4 - 5.77 and a copy 4.8; with 8-bit moments 298 us = 5.4 TB/s; 1.28e9 bf16 elements with
-// 8-bit moments 2.43 ms = 5.3 TB/s (the same streams without arithmetic: 2.33 - 2.53 ms), with f32 weights beside them and 32-bit
-// moments 6.59 ms = 5.4 TB/s.  Counted traffic is 1.00 - 1.02 of those bytes.  24 vector instructions per element (8 bits) are
-// below a third of the time.  All accesses stream (non-temporal: 493 against 535 us at 1e8).  m and v are formed by separate products and sums (no fma), so that they -- and
+// moments, 10 B with bf16 weights and 8-bit moments.  Reached (MI355X): 1e8 f32 elements 474 us = 5.9 TB/s, where four read and three
+// write streams without arithmetic reach 5.4 - 5.77 and a copy 4.8; with 8-bit moments 304 us = 5.3 TB/s; 1.28e9 bf16 elements with
+// 8-bit moments 2.41 ms = 5.3 TB/s (the same streams without arithmetic: 2.33 - 2.53 ms), with f32 weights beside them and 32-bit
+// moments 6.52 ms = 5.5 TB/s.  Counted traffic is 1.00 - 1.02 of those bytes.  24 vector instructions per element (8 bits) are
+// below a third of the time.  All accesses stream (non-temporal: 8 % at 1e8).  m and v are formed by separate products and sums (no fma), so that they -- and
 // with them the 8-bit codes -- do not depend on what a compiler contracts.
 #include "tensors.hpp"
 
@@ -18,42 +18,26 @@ namespace {
 constexpr int kThreads = 256;
 
 // Tensors are aligned to their elements only, the arrays of the state to 16 bytes; global memory takes wide accesses at any address.
-template <int BYTES, int ALIGN> struct Wide;
-#define TS_WIDE(bytes, align) \
-	template <> struct Wide<bytes, align> { typedef uint32_t type __attribute__((ext_vector_type(bytes / 4), aligned(align))); };
-TS_WIDE(16, 16) TS_WIDE(16, 4) TS_WIDE(16, 2) TS_WIDE(8, 8) TS_WIDE(8, 2)
-#undef TS_WIDE
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <class T, int ALIGN> struct Aligned;
+template <int ALIGN> struct Aligned<u32x4, ALIGN> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Aligned<u32x4, 16> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(16))); };
+template <> struct Aligned<u32x4, 4> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4))); };
+template <int ALIGN> struct Aligned<u32x2, ALIGN> { typedef uint32_t type __attribute__((ext_vector_type(2), aligned(2))); };
+template <> struct Aligned<u32x2, 8> { typedef uint32_t type __attribute__((ext_vector_type(2), aligned(8))); };
 
-// BYTES bytes (8, 16, 32) from / to global memory
-template <int BYTES, int ALIGN> __device__ inline void fetch(const void* p, uint32_t (&x)[BYTES / 4])
+template <int ALIGN, class T> __device__ inline void fetch(const void* p, T& x)
 {
-	constexpr int W = BYTES < 16 ? BYTES : 16;
-	typedef typename Wide<W, ALIGN>::type T;
-#pragma unroll
-	for (int k = 0; k < BYTES / W; k++) {
-		const T t = __builtin_nontemporal_load(static_cast<const T*>(p) + k);
-#pragma unroll
-		for (int j = 0; j < W / 4; j++) x[k * W / 4 + j] = t[j];
-	}
+	x = __builtin_nontemporal_load(static_cast<const typename Aligned<T, ALIGN>::type*>(p));
 }
-template <int BYTES, int ALIGN> __device__ inline void put(void* p, const uint32_t (&x)[BYTES / 4])
+template <int ALIGN, class T> __device__ inline void put(void* p, T x)
 {
-	constexpr int W = BYTES < 16 ? BYTES : 16;
-	typedef typename Wide<W, ALIGN>::type T;
-#pragma unroll
-	for (int k = 0; k < BYTES / W; k++) {
-		T t;
-#pragma unroll
-		for (int j = 0; j < W / 4; j++) t[j] = x[k * W / 4 + j];
-		__builtin_nontemporal_store(t, static_cast<T*>(p) + k);
-	}
+	__builtin_nontemporal_store((typename Aligned<T, ALIGN>::type) x, static_cast<typename Aligned<T, ALIGN>::type*>(p));
 }
 
 __device__ inline float bits_float(uint32_t b) { return __builtin_bit_cast(float, b); }
 __device__ inline uint32_t float_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
-
-// V elements of a tensor as they lie in memory: f32 one to a word, 16 bits two to a word (in the first half of the words)
-template <int V> struct Raw { uint32_t w[V]; };
 
 __device__ inline float widen16(uint32_t h, int type)
 {
@@ -64,48 +48,62 @@ __device__ inline uint32_t narrow16(float f, int type)
 	return type == T_BF16 ? (uint32_t) __builtin_bit_cast(uint16_t, (__bf16) f) : (uint32_t) __builtin_bit_cast(uint16_t, (_Float16) f);
 }
 
-// elements i .. i+V-1 of a tensor of n; what lies behind its end reads as zero
-template <int V> __device__ inline void load(const void* base, uint64_t i, uint64_t n, int type, Raw<V>& x)
+// What is known of a tensor where a tile of it is taken: nothing, or that the whole tile lies in it and how wide its elements are.
+enum Kind { ANY, WIDE, HALF };
+
+// V elements of a tensor on their way.  Every load has registers of its own: where two branches load into the same ones the compiler copies,
+// and waits for each load before it issues the next (1e8 f32 elements with 32-bit moments: 487 us so, 474 like this).
+template <int V> struct Raw;
+template <> struct Raw<8> { u32x4 a, b; };                                   // f32: a, b; 16 bits: a
+template <> struct Raw<4> { u32x4 a; u32x2 b; };                             // f32: a; 16 bits: b
+
+// elements i .. i+V-1 of a tensor of n, if all of them exist
+template <int V, Kind K = ANY> __device__ inline void load(const void* base, uint64_t i, uint64_t n, int type, Raw<V>& x)
 {
-	if (i + V <= n) {
-		if (type == T_F32) fetch<V * 4, 4>(static_cast<const float*>(base) + i, x.w);
-		else {
-			uint32_t h[V / 2];
-			fetch<V * 2, 2>(static_cast<const uint16_t*>(base) + i, h);
+	if (K == ANY && i + V > n) return;
+	const bool wide = K == ANY ? type == T_F32 : K == WIDE;
+	const char* at = static_cast<const char*>(base) + (i << (wide ? 2 : 1));
+	if constexpr (V == 8) {
+		fetch<2>(at, x.a);
+		if (wide) fetch<4>(at + 16, x.b);
+	} else {
+		if (wide) fetch<4>(at, x.a);
+		if (!wide) fetch<2>(at, x.b);
+	}
+}
+// ... as f32.  Where a tensor ends inside of them they are loaded here, one by one; what lies behind its end is zero.
+template <int V, Kind K = ANY> __device__ inline void widen(const Raw<V>& r, const void* base, uint64_t i, uint64_t n, int type, float (&x)[V])
+{
+	if (K == ANY && i + V > n) {
 #pragma unroll
-			for (int j = 0; j < V / 2; j++) x.w[j] = h[j];
+		for (int j = 0; j < V; j++) {
+			x[j] = 0;
+			if (i + j < n) x[j] = type == T_F32 ? static_cast<const float*>(base)[i + j] : widen16(static_cast<const uint16_t*>(base)[i + j], type);
 		}
+	} else if (K == ANY ? type == T_F32 : K == WIDE) {
+#pragma unroll
+		for (int j = 0; j < V; j++) x[j] = bits_float(j < 4 ? r.a[j] : r.b[j & 3]);
 	} else {
+		uint32_t h[V / 2];
 #pragma unroll
-		for (int j = 0; j < V; j++) x.w[j] = 0;
+		for (int j = 0; j < V / 2; j++) {
+			if constexpr (V == 8) h[j] = r.a[j];
+			else h[j] = r.b[j];
+		}
+		if (type == T_BF16) {
 #pragma unroll
-		for (int j = 0; j < V; j++)
-			if (i + j < n) {
-				if (type == T_F32) x.w[j] = static_cast<const uint32_t*>(base)[i + j];
-				else x.w[j / 2] |= (uint32_t) static_cast<const uint16_t*>(base)[i + j] << 16 * (j & 1);
-			}
+			for (int j = 0; j < V; j += 2) { x[j] = bits_float(h[j / 2] << 16); x[j + 1] = bits_float(h[j / 2] & 0xffff0000u); }
+		} else {
+#pragma unroll
+			for (int j = 0; j < V; j += 2) { x[j] = widen16(h[j / 2] & 0xffff, T_F16); x[j + 1] = widen16(h[j / 2] >> 16, T_F16); }
+		}
 	}
 }
-template <int V> __device__ inline void widen(const Raw<V>& r, int type, float (&x)[V])
-{
-	if (type == T_F32) {
-#pragma unroll
-		for (int j = 0; j < V; j++) x[j] = bits_float(r.w[j]);
-	} else if (type == T_BF16) {
-#pragma unroll
-		for (int j = 0; j < V; j += 2) { x[j] = bits_float(r.w[j / 2] << 16); x[j + 1] = bits_float(r.w[j / 2] & 0xffff0000u); }
-	} else {
-#pragma unroll
-		for (int j = 0; j < V; j += 2) { x[j] = widen16(r.w[j / 2] & 0xffff, T_F16); x[j + 1] = widen16(r.w[j / 2] >> 16, T_F16); }
-	}
-}
-template <int V> __device__ inline void store32(float* base, uint64_t i, uint64_t n, const float (&x)[V])
+template <int V, int ALIGN> __device__ inline void store32(float* base, uint64_t i, uint64_t n, const float (&x)[V])
 {
 	if (i + V <= n) {
-		uint32_t w[V];
 #pragma unroll
-		for (int j = 0; j < V; j++) w[j] = float_bits(x[j]);
-		put<V * 4, 4>(base + i, w);
+		for (int j = 0; j < V; j += 4) put<ALIGN>(base + i + j, u32x4{float_bits(x[j]), float_bits(x[j + 1]), float_bits(x[j + 2]), float_bits(x[j + 3])});
 	} else {
 #pragma unroll
 		for (int j = 0; j < V; j++)
@@ -114,8 +112,10 @@ template <int V> __device__ inline void store32(float* base, uint64_t i, uint64_
 }
 template <int V> __device__ inline void store16(uint16_t* base, uint64_t i, uint64_t n, const uint32_t (&h)[V / 2])
 {
-	if (i + V <= n) put<V * 2, 2>(base + i, h);
-	else {
+	if (i + V <= n) {
+		if constexpr (V == 8) put<2>(base + i, u32x4{h[0], h[1], h[2], h[3]});
+		else put<2>(base + i, u32x2{h[0], h[1]});
+	} else {
 #pragma unroll
 		for (int j = 0; j < V; j++)
 			if (i + j < n) base[i + j] = (uint16_t) (h[j / 2] >> 16 * (j & 1));
@@ -168,12 +168,11 @@ struct Step {
 	bool go, stochastic, careful;
 };
 
-__device__ inline Step step_of(const AdamwArgs& a, long long t)
+__device__ inline Step step_of(const AdamwArgs& a, long long t, float scale, double lr)
 {
 	Step s{};
 	// a scale or a step size that is not finite: the step is rejected as a whole, nothing changes and nothing is counted
-	const double lr = a.step_size_dev ? (double) *a.step_size_dev : a.step_size;
-	s.scale = a.grad_scale ? *a.grad_scale : 1.0f;
+	s.scale = scale;
 	s.go = __builtin_isfinite(s.scale) && __builtin_isfinite(lr);
 	if (!s.go) return s;
 	double p1 = 1, p2 = 1, q1 = a.beta1, q2 = a.beta2;       // b^t by squaring, in f64: 1 - b2^t loses ten bits at t = 1
@@ -212,9 +211,9 @@ __device__ inline void update(const Step& s, float decay, float g, float& m, flo
 // the upper half of f32, so the word's 16 bits are added to the lower half and cut off with it)
 template <int V> __device__ inline void put_weights(const Step& s, void* param, uint64_t i, uint64_t n, int ptype, float* master, const float (&w)[V], uint32_t word)
 {
-	if (ptype == T_F32) { store32<V>(static_cast<float*>(param), i, n, w); return; }
+	if (ptype == T_F32) { store32<V, 4>(static_cast<float*>(param), i, n, w); return; }
+	if (master) store32<V, 16>(master, i, n, w);
 	uint32_t h[V / 2];
-	if (master) store32<V>(master, i, n, w);
 	if (ptype == T_F16) {
 #pragma unroll
 		for (int j = 0; j < V; j += 2) h[j / 2] = narrow16(w[j], T_F16) | narrow16(w[j + 1], T_F16) << 16;
@@ -256,7 +255,7 @@ __device__ inline uint32_t scale_byte(uint32_t top, int at)
 
 constexpr int kLane = 8;                                                     // elements of a block per lane
 
-template <bool SECOND> __device__ inline void encode(const float (&x)[kLane], uint32_t byte, uint32_t word, uint32_t (&c)[2])
+template <bool SECOND> __device__ inline void encode(const float (&x)[kLane], uint32_t byte, uint32_t word, u32x2& c)
 {
 	const float scale = scale_float(byte);
 	// a second moment above zero stays above zero (the least code, 2^-16): m / (sqrt(0) + eps) would be a jump
@@ -271,11 +270,10 @@ template <bool SECOND> __device__ inline void encode(const float (&x)[kLane], ui
 	TS_ENC(0, 0); TS_ENC(1, 1); TS_ENC(2, 2); TS_ENC(3, 3);
 	TS_ENC(4, 0); TS_ENC(5, 1); TS_ENC(6, 2); TS_ENC(7, 3);
 #undef TS_ENC
-	c[0] = (uint32_t) out[0];
-	c[1] = (uint32_t) out[1];
+	c = u32x2{(uint32_t) out[0], (uint32_t) out[1]};
 }
 
-template <bool SECOND> __device__ inline void decode(const uint32_t (&c)[2], float scale, float (&x)[kLane])
+template <bool SECOND> __device__ inline void decode(u32x2 c, float scale, float (&x)[kLane])
 {
 #pragma unroll
 	for (int k = 0; k < 2; k++) {
@@ -315,7 +313,8 @@ __device__ inline uint64_t word_of(const Step& s, uint64_t element) { return fin
 // A tile with moments in 32 bits: four elements per lane (16 B of every f32 array), U such groups in flight.
 template <int TILE> struct Tile32 {
 	static constexpr int V = 4, U = TILE / kThreads / V;
-	Raw<V> g[U], w[U], m[U], v[U];
+	Raw<V> g[U], w[U];
+	u32x4 m[U], v[U];
 	__device__ static uint64_t at(uint64_t first, int u) { return first + (u * kThreads + threadIdx.x) * V; }
 	__device__ void load(const AdamwArgs& a, const Place& p, uint64_t first)
 	{
@@ -325,8 +324,8 @@ template <int TILE> struct Tile32 {
 			if (i >= p.n) continue;
 			sqn::load<V>(p.grad, i, p.n, p.gtype, g[u]);
 			sqn::load<V>(p.weights(), i, p.n, p.wtype(), w[u]);
-			fetch<V * 4, 16>(static_cast<float*>(a.m) + p.state + i, m[u].w);
-			fetch<V * 4, 16>(static_cast<float*>(a.v) + p.state + i, v[u].w);
+			fetch<16>(static_cast<float*>(a.m) + p.state + i, m[u]);
+			fetch<16>(static_cast<float*>(a.v) + p.state + i, v[u]);
 		}
 	}
 	__device__ void work(const AdamwArgs& a, const Step& s, const Place& p, uint64_t first)
@@ -337,18 +336,18 @@ template <int TILE> struct Tile32 {
 			const uint64_t i = at(first, u);
 			if (i >= p.n) continue;
 			float fg[V], fw[V], fm[V], fv[V];
-			widen<V>(g[u], p.gtype, fg);
-			widen<V>(w[u], p.wtype(), fw);
+			widen<V>(g[u], p.grad, i, p.n, p.gtype, fg);
+			widen<V>(w[u], p.weights(), i, p.n, p.wtype(), fw);
 			uint32_t word = 0;
 			if (s.stochastic) word = (uint32_t) word_of(s, p.state + i) + (uint32_t) (i & 7) * kLaneStep;
 #pragma unroll
 			for (int j = 0; j < V; j++) {
-				fm[j] = bits_float(m[u].w[j]);
-				fv[j] = bits_float(v[u].w[j]);
+				fm[j] = bits_float(m[u][j]);
+				fv[j] = bits_float(v[u][j]);
 				update(s, decay, fg[j] * s.scale, fm[j], fv[j], fw[j]);
 			}
-			store32<V>(static_cast<float*>(a.m) + p.state, i, p.n, fm);
-			store32<V>(static_cast<float*>(a.v) + p.state, i, p.n, fv);
+			store32<V, 16>(static_cast<float*>(a.m) + p.state, i, p.n, fm);
+			store32<V, 16>(static_cast<float*>(a.v) + p.state, i, p.n, fv);
 			put_weights<V>(s, p.param, i, p.n, p.ptype, p.master, fw, word);
 		}
 	}
@@ -358,7 +357,7 @@ template <int TILE> struct Tile32 {
 template <int TILE> struct Tile8 {
 	static constexpr int V = kLane, U = TILE / kThreads / V;
 	Raw<V> g[U], w[U];
-	uint32_t m[U][2], v[U][2];
+	u32x2 m[U], v[U];
 	uint8_t ms[U], vs[U];
 	__device__ static uint64_t at(uint64_t first, int u) { return first + (u * kThreads + threadIdx.x) * V; }
 	__device__ static bool outside(uint64_t i, uint64_t n) { return (i & ~(uint64_t) (kStateBlock - 1)) >= n; }   // the same for the 16 lanes of a block
@@ -372,8 +371,8 @@ template <int TILE> struct Tile8 {
 			vs[u] = a.v_scale[(p.state + i) / kStateBlock];
 			sqn::load<V>(p.grad, i, p.n, p.gtype, g[u]);
 			sqn::load<V>(p.weights(), i, p.n, p.wtype(), w[u]);
-			fetch<V, V>(static_cast<uint8_t*>(a.m) + p.state + i, m[u]);
-			fetch<V, V>(static_cast<uint8_t*>(a.v) + p.state + i, v[u]);
+			fetch<V>(static_cast<uint8_t*>(a.m) + p.state + i, m[u]);
+			fetch<V>(static_cast<uint8_t*>(a.v) + p.state + i, v[u]);
 		}
 	}
 	__device__ void work(const AdamwArgs& a, const Step& s, const Place& p, uint64_t first)
@@ -385,8 +384,8 @@ template <int TILE> struct Tile8 {
 			const uint64_t i = at(first, u);
 			if (outside(i, p.n)) continue;
 			float fg[V], fw[V], fm[V], fv[V];
-			widen<V>(g[u], p.gtype, fg);
-			widen<V>(w[u], p.wtype(), fw);
+			widen<V>(g[u], p.grad, i, p.n, p.gtype, fg);
+			widen<V>(w[u], p.weights(), i, p.n, p.wtype(), fw);
 			decode<false>(m[u], scale_float(ms[u]), fm);
 			decode<true>(v[u], scale_float(vs[u]), fv);
 			const uint64_t word = word_of(s, p.state + i);
@@ -407,11 +406,11 @@ template <int TILE> struct Tile8 {
 					if (fm[j] != fm[j]) tm = __builtin_inff();
 			}
 			const uint32_t om = scale_byte(row_reduce(float_bits(tm), larger), 7), ov = scale_byte(tv, 14);
-			uint32_t c[2];
+			u32x2 c;
 			encode<false>(fm, om, (uint32_t) word, c);
-			put<V, V>(static_cast<uint8_t*>(a.m) + p.state + i, c);
+			put<V>(static_cast<uint8_t*>(a.m) + p.state + i, c);
 			encode<true>(fv, ov, (uint32_t) (word >> 32), c);
-			put<V, V>(static_cast<uint8_t*>(a.v) + p.state + i, c);
+			put<V>(static_cast<uint8_t*>(a.v) + p.state + i, c);
 			if ((threadIdx.x & 15) == 0) {
 				a.m_scale[(p.state + i) / kStateBlock] = (uint8_t) om;
 				a.v_scale[(p.state + i) / kStateBlock] = (uint8_t) ov;
@@ -428,6 +427,9 @@ template <template <int> class Tile, int TILE, int N> __global__ __launch_bounds
 {
 	const AdamwArgs& a = table.a;
 	Cursor<Table<AdamwArgs, N>> cursor(table, blockIdx.x);
+	const long long count = a.count[0] + 1;                 // read in front of every store: scalar loads
+	const float scale = a.grad_scale ? *a.grad_scale : 1.0f;
+	const double lr = a.step_size_dev ? (double) *a.step_size_dev : a.step_size;
 	Tile<TILE> t;
 	Place p{};
 	uint64_t first = 0;
@@ -439,8 +441,7 @@ template <template <int> class Tile, int TILE, int N> __global__ __launch_bounds
 	};
 	uint32_t tile = blockIdx.x;
 	if (tile < a.tiles) load(tile);
-	const long long count = a.count[0] + 1;
-	const Step s = step_of(a, count);
+	const Step s = step_of(a, count, scale, lr);
 	if (!s.go) return;
 	while (tile < a.tiles) {
 		t.work(a, s, p, first);
@@ -461,7 +462,8 @@ template <template <int> class Tile, int TILE, int N> __global__ __launch_bounds
 }
 
 // ---- the norm ------------------------------------------------------------------------------------------------------------------------
-// Bound by reading: 1.28e9 bf16 elements in 377 us = 6.8 TB/s, what the card reads at; below 1e7 elements by its two launches (9.4 us).
+// Bound by reading: 1.28e9 bf16 elements in 379 us = 6.75 TB/s, what the card reads at; below 1e7 elements by its two launches.  Tiles that
+// lie in their tensor as a whole take code without a branch between its loads (1e8 f32 elements: 67.7 us, 72 with branches).
 // Squares are summed in f64: f32 gradients reach 3e38, whose square is past f32, and 1e9 of them add up.  The order is fixed by the sizes
 // alone -- lane, wave, workgroup, then the partial sums by one workgroup -- so that the same gradients give the same bits.
 template <int THREADS> __device__ inline double block_sum(double x)
@@ -486,28 +488,36 @@ __device__ inline void verdict(double sum, double grad_scale, double max_norm, f
 	out[1] = !finite ? __builtin_nanf("") : (float) (norm > max_norm ? grad_scale * (max_norm / norm) : grad_scale);
 }
 
-template <int TILE, int N> __global__ __launch_bounds__(kThreads) void k_norm(const Table<NormArgs, N> table)
+template <int TILE, Kind K> __device__ inline double squares(const void* grad, uint64_t first, uint64_t n, int type, double sum)
 {
 	constexpr int V = 8, U = TILE / kThreads / V;
+	Raw<V> r[U];
+#pragma unroll
+	for (int u = 0; u < U; u++) load<V, K>(grad, first + (u * kThreads + threadIdx.x) * V, n, type, r[u]);
+#pragma unroll
+	for (int u = 0; u < U; u++) {
+		const uint64_t i = first + (u * kThreads + threadIdx.x) * V;
+		if (K == ANY && i >= n) continue;
+		float g[V];
+		widen<V, K>(r[u], grad, i, n, type, g);
+#pragma unroll
+		for (int j = 0; j < V; j++) sum = fma((double) g[j], (double) g[j], sum);
+	}
+	return sum;
+}
+
+template <int TILE, int N> __global__ __launch_bounds__(kThreads) void k_norm(const Table<NormArgs, N> table)
+{
 	const NormArgs& a = table.a;
 	double sum = 0;
 	Cursor<Table<NormArgs, N>> cursor(table, blockIdx.x);
 	for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
 		const TensorEntry& e = cursor.at(tile);
-		const uint64_t n = e.info & kCountMask, first = (uint64_t) (tile - e.tile0) * TILE + threadIdx.x * V;
+		const uint64_t n = e.info & kCountMask, first = (uint64_t) (tile - e.tile0) * TILE;
 		const int type = (int) (e.info >> 58) & 3;
-		Raw<V> r[U];
-#pragma unroll
-		for (int u = 0; u < U; u++)
-			if (first + u * kThreads * V < n) load<V>(e.grad, first + u * kThreads * V, n, type, r[u]);
-#pragma unroll
-		for (int u = 0; u < U; u++) {
-			if (first + u * kThreads * V >= n) continue;
-			float g[V];
-			widen<V>(r[u], type, g);
-#pragma unroll
-			for (int j = 0; j < V; j++) sum = fma((double) g[j], (double) g[j], sum);
-		}
+		if (first + TILE > n) sum = squares<TILE, ANY>(e.grad, first, n, type, sum);
+		else if (type == T_F32) sum = squares<TILE, WIDE>(e.grad, first, n, type, sum);
+		else sum = squares<TILE, HALF>(e.grad, first, n, type, sum);
 	}
 	sum = block_sum<kThreads>(sum);
 	if (threadIdx.x) return;
@@ -552,7 +562,8 @@ void launch_adamw(hipStream_t st, int bits, int tile, int grid, const Table<Adam
 }
 void launch_norm(hipStream_t st, int tile, int grid, const Table<NormArgs, kEntries>& t)
 {
-	if (tile != kTileSmall) k_norm<kTile8, kEntries><<<grid, kThreads, 0, st>>>(t);
+	if (tile == kTileNorm) k_norm<kTileNorm, kEntries><<<grid, kThreads, 0, st>>>(t);
+	else if (tile == kTileNormMid) k_norm<kTileNormMid, kEntries><<<grid, kThreads, 0, st>>>(t);
 	else if (t.a.entries > kFewEntries) k_norm<kTileSmall, kEntries><<<grid, kThreads, 0, st>>>(t);
 	else k_norm<kTileSmall, kFewEntries><<<grid, kThreads, 0, st>>>(few(t));
 }
