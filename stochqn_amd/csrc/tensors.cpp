@@ -22,8 +22,8 @@ using namespace sqn;
 namespace {
 
 // Most workgroups per compute unit.  Measured at 1.28e9 elements: 32-bit moments 6.51 ms with 8, 6.50 with 16 (at 7.7e6 elements
-// 43.3 and 40.3 us); 8-bit moments 2.53 ms with 8, 2.47 with
-// 16, 2.44 with 32, 2.46 with 64; the norm 466 us with 4, 377 with 8, 379 with 16.
+// 43.3 and 40.3 us); 8-bit moments 2.53 ms with 8, 2.47 with 16, 2.44 with 32, 2.46 with 64; the norm 466 us with 4, 377 with 8,
+// 379 with 16.
 constexpr int kPerUnit32 = 16, kPerUnit8 = 32, kPerUnitNorm = 8;
 
 struct Range { const char* at; size_t bytes; };                              // of device memory
