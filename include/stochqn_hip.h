@@ -285,7 +285,7 @@ size_t stochqn_hip_tensors_state(const stochqn_hip_tensors *tensors, size_t offs
  * that is not finite makes out[1] NaN, which the step below takes as "reject".  Sums in f64, in an order that depends on the sizes
  * alone.  work: stochqn_hip_tensors_norm_work() doubles that nothing else uses until the call's work is done.  With a communicator or
  * reducer installed the tensors are this rank's share and the sum is over all ranks (one double; every rank makes the call), like
- * every other sum of the library; work[0] holds it afterwards.  Returns 0 or -1000. */
+ * every other sum of the library; work[0] holds it afterwards.  out, work and the tensors do not overlap.  Returns 0 or -1000. */
 size_t stochqn_hip_tensors_norm_work(const stochqn_hip_tensors *tensors);
 int stochqn_hip_tensors_norm(stochqn_hip_tensors *tensors, double grad_scale, double max_norm, float out[], double work[], void *hip_stream);
 
@@ -305,7 +305,8 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors *tensors, double grad_scale, do
  *   decay             one byte per tensor, 0: no weight decay for it; NULL: all decay
  *   count             two int64: steps taken; zero (arrivals within a step)
  *   work              4096 bytes, aligned to 8, zero: arrivals as well
- * m, v, master aligned to 16 bytes.  eps >= 2^-126.  No two arrays that the step writes may overlap, nor a gradient with one.
+ * m, v, master aligned to 16 bytes.  eps >= 2^-126.  No two arrays that the step writes may overlap, nor a gradient,
+ * step_size_dev or grad_scale with one.
  * step:  grads: as many tensors, of the same sizes, f32 / bf16 / f16 each; step_size_dev (nullable): a float on the device in place of
  * step_size (schedules in a captured graph); grad_scale (nullable = 1): a float on the device, out + 1 of the norm.  If either
  * is not finite the step is rejected: nothing is written and nothing counted -- the guard of take_step, left on the device.  Returns 0 or

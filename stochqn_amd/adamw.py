@@ -62,7 +62,7 @@ def _scalar(t, device, what):
     """Address of a device tensor of one float32 (None: none)."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device or t.is_neg():
         raise ValueError("'%s' has to be a float32 tensor of one element on %s." % (what, device))
     return t.data_ptr()
 
@@ -70,8 +70,8 @@ def _scalar(t, device, what):
 class TensorList:
     """Tensors of one device (parameters, or their gradients) as the library takes them: contiguous, float32 / bfloat16 / float16 each.
 
-    The list keeps the tensors alive.  `rebind(tensors)` names other ones of the same sizes and types; a graph that was captured before
-    goes on with those it saw."""
+    The list keeps the tensors and their memory alive.  `rebind(tensors)` names other ones of the same sizes and types; a graph that was
+    captured before goes on with those it saw, which have to be kept alive for it."""
 
     _handle = None
 
@@ -90,6 +90,7 @@ class TensorList:
         self.sizes = [t.numel() for t in self.tensors]
         self.dtypes = [t.dtype for t in self.tensors]
         self._at = self._addresses(self.tensors)
+        self._memory = [t.untyped_storage() for t in self.tensors]       # a tensor that is given other memory (`.data = ...`) lets go of it
         self._lib = _library()
         self._handle = self._lib.stochqn_hip_tensors_create(n, (C.c_void_p * n)(*self._at), (C.c_size_t * n)(*self.sizes),
                                                             (C.c_int * n)(*[types[d] for d in self.dtypes]))
@@ -100,12 +101,12 @@ class TensorList:
     def _addresses(self, tensors):
         at = []
         for t, n, dtype in zip(tensors, self.sizes, self.dtypes):
-            if t.numel() != n or t.dtype != dtype:
+            if getattr(t, "dtype", None) != dtype or t.numel() != n:
                 raise ValueError("the tensors have other sizes or types than the list's.")
             if t.get_device() != self._index:
                 raise ValueError("tensors have to be on one GPU.")
-            if not t.is_contiguous():
-                raise ValueError("tensors have to be contiguous.")
+            if t.layout != torch.strided or not t.is_contiguous() or t.is_neg():
+                raise ValueError("tensors have to be dense and contiguous, and no views that negate.")
             at.append(t.data_ptr())
         return at
 
@@ -119,6 +120,7 @@ class TensorList:
             if self._lib.stochqn_hip_tensors_rebind(self._handle, (C.c_void_p * len(at))(*at)) != 0:
                 raise ValueError("the library refused the tensors (its reason is on stderr).")
             self._at = at
+            self._memory = [t.untyped_storage() for t in tensors]
         self.tensors = tensors
 
     def __len__(self):
@@ -170,6 +172,7 @@ class AdamW_free:
         assert not (master and stochastic)
         self.params = params if isinstance(params, TensorList) else TensorList(params)
         self.tensors = list(self.params.tensors)        # what the steps write, whatever the list is rebound to later
+        self._at, self._memory = list(self.params._at), list(self.params._memory)
         assert not (stochastic and torch.float16 in self.params.dtypes)
         if decay is not None and len(decay) != len(self.params):
             raise ValueError("'decay' has to have one truth value per tensor.")
@@ -213,7 +216,9 @@ class AdamW_free:
 
     def update_gradient(self, gradient):
         """Name the gradients of the coming steps: tensors (or a TensorList) in the order of the parameters.  Nothing is copied: the steps
-        read what the tensors hold by then."""
+        read what the tensors hold by then.  The parameters have to be where they were when the object was made (no `.data = ...`)."""
+        if [t.data_ptr() for t in self.tensors] != self._at:
+            raise ValueError("a parameter has other memory than when the optimizer was made: make a new one, with the old one's state.")
         if isinstance(gradient, TensorList):
             if gradient.sizes != self.params.sizes or gradient.device != self.params.device:
                 raise ValueError("the gradients have other sizes or another device than the parameters.")

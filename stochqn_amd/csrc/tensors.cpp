@@ -28,6 +28,13 @@ constexpr int kPerUnit32 = 16, kPerUnit8 = 32, kPerUnitNorm = 8;
 
 struct Range { const char* at; size_t bytes; };                              // of device memory
 bool before(const Range& a, const Range& b) { return a.at < b.at; }
+bool overlap(const Range& a, const Range& b) { return a.at < b.at + b.bytes && b.at < a.at + a.bytes; }
+// with one of the sorted ranges that do not overlap each other
+bool overlaps(const std::vector<Range>& sorted, const Range& r)
+{
+	const auto after = std::upper_bound(sorted.begin(), sorted.end(), r, before);
+	return (after != sorted.end() && overlap(r, *after)) || (after != sorted.begin() && overlap(r, *(after - 1)));
+}
 
 struct Item { void* p; size_t n; int type; };
 
@@ -260,8 +267,15 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors* t, double grad_scale, double m
 		int device = t->device;
 		check_aligned(out, sizeof(float), "out");
 		check_aligned(work, sizeof(double), "work");
-		check_memory(out, 2 * sizeof(float), device, "out");
-		check_memory(work, stochqn_hip_tensors_norm_work(t) * sizeof(double), device, "work");
+		const Range result{reinterpret_cast<const char*>(out), 2 * sizeof(float)};
+		const Range scratch{reinterpret_cast<const char*>(work), stochqn_hip_tensors_norm_work(t) * sizeof(double)};
+		check_memory(out, result.bytes, device, "out");
+		check_memory(work, scratch.bytes, device, "work");
+		if (overlap(result, scratch)) refuse("out overlaps work");
+		for (const Item& it : t->items) {
+			const Range r{static_cast<const char*>(it.p), it.n * type_size(it.type)};
+			if (it.n && (overlap(r, result) || overlap(r, scratch))) refuse("out or work overlaps a tensor");
+		}
 		OnDevice on(device);
 		hipStream_t st = check_stream(hip_stream, device);
 		(void) hipGetLastError();                                  // somebody else's: only what the launches below leave counts
@@ -365,14 +379,14 @@ int stochqn_hip_adamw_step(stochqn_hip_adamw* o, stochqn_hip_tensors* grads, dou
 			for (size_t i = 0; i < g.size(); i++) {
 				if (!g[i].n) continue;
 				const Range r{static_cast<char*>(g[i].p), g[i].n * type_size(g[i].type)};
-				const auto after = std::upper_bound(o->written.begin(), o->written.end(), r, before);
-				if ((after != o->written.end() && r.at + r.bytes > after->at) || (after != o->written.begin() && (after - 1)->at + (after - 1)->bytes > r.at))
-					refuse("gradient " + std::to_string(i) + " overlaps an array that the step writes");
+				if (overlaps(o->written, r)) refuse("gradient " + std::to_string(i) + " overlaps an array that the step writes");
 			}
 			o->checked = grads->version;
 		}
 		check_scalar(step_size_dev, o->device, "step_size");
 		check_scalar(grad_scale, o->device, "grad_scale");
+		for (const float* scalar : {step_size_dev, grad_scale})             // read by every workgroup, whatever others have written by then
+			if (scalar && overlaps(o->written, {reinterpret_cast<const char*>(scalar), sizeof(float)})) refuse("step_size or grad_scale overlaps an array that the step writes");
 		OnDevice on(o->device);
 		hipStream_t st = check_stream(hip_stream, o->device);
 		(void) hipGetLastError();

@@ -314,6 +314,39 @@ static void refusals()
 	stochqn_hip_adamw_destroy(o);
 }
 
+// what a call reads or writes besides the tensors does not overlap what it writes
+static void overlaps_in_a_call()
+{
+	Lists l({1000, 50, 0, 7});
+	const size_t blocks = stochqn_hip_tensors_state(l.params, nullptr) / 128;
+	for (int bits : {32, 8}) {
+		stochqn_hip_adamw_setup s = l.setup(bits);
+		stochqn_hip_adamw* o = stochqn_hip_adamw_create(l.params, &s);
+		CHECK(o);
+		float* apart = (float*) device_block(8);
+		std::vector<void*> written{l.p[0], l.p[3], s.m, (char*) s.m + blocks * 128 * bits / 8 - 4, s.v, s.master, s.count, (char*) s.count + 12, s.work, (char*) s.work + 4092};
+		if (bits == 8) written.push_back((void*) (((uintptr_t) s.m_scale + 3) & ~(uintptr_t) 3));
+		g_launches.clear();
+		for (void* p : written) {
+			CHECK(stochqn_hip_adamw_step(o, l.grads, 0.1, (float*) p, apart, nullptr) == -1000);
+			CHECK(stochqn_hip_adamw_step(o, l.grads, 0.1, apart, (float*) p, nullptr) == -1000);
+		}
+		CHECK(g_launches.empty());
+		CHECK(stochqn_hip_adamw_step(o, l.grads, 0.1, apart, apart + 1, nullptr) == 0 && stochqn_hip_adamw_step(o, l.grads, 0.1, apart, apart, nullptr) == 0);
+		CHECK(stochqn_hip_adamw_step(o, l.grads, 0.1, (float*) l.g[0], nullptr, nullptr) == 0);        // the step only reads gradients
+		stochqn_hip_adamw_destroy(o);
+	}
+	const size_t doubles = stochqn_hip_tensors_norm_work(l.grads);
+	char* work = (char*) device_block(8 * doubles + 8);
+	float* out = (float*) device_block(16);
+	const auto norm = [&](void* to, void* with) { return stochqn_hip_tensors_norm(l.grads, 1, 1, (float*) to, (double*) with, nullptr); };
+	g_launches.clear();
+	CHECK(norm(work, work) == -1000 && norm(work + 8 * doubles - 4, work) == -1000 && norm(l.g[0], work) == -1000 && norm((char*) l.g[1] + 4, work) == -1000);
+	CHECK(norm(out, (void*) (((uintptr_t) l.g[0] + 7) & ~(uintptr_t) 7)) == -1000);
+	CHECK(g_launches.empty());
+	CHECK(norm(work + 8 * doubles, work) == 0 && norm(out, work) == 0 && norm(l.p[0], work) == 0);
+}
+
 // A list that two optimizers read while a third thread rebinds it and a fourth takes its norm: every table is of one binding or the other.
 static void concurrent()
 {
@@ -368,6 +401,7 @@ int main(int argc, char**)
 		}
 	}
 	refusals();
+	overlaps_in_a_call();
 	std::printf("ok\n");
 	return 0;
 }

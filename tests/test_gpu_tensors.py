@@ -577,6 +577,71 @@ def test_the_first_steps_with_adamw_the_rest_with_sqn():
     assert torch.isfinite(x).all() and float((d * x * x).sum()) < loss[0]
 
 
+def test_memory_that_a_step_or_a_norm_both_reads_and_writes_is_refused():
+    sq = stochqn()
+    one, p = torch.ones(1, device="cuda"), torch.ones(300, device="cuda")
+    g = torch.ones(300, device="cuda")
+    opt = sq.AdamW_free([p, one], state_bits=8, master=True)
+    grads = sq.TensorList([g, torch.ones(1, device="cuda")])
+    opt.update_gradient(grads)
+    for scalar in (one, p[7:8], opt.master[3:4], opt.m[:4].view(torch.float32), opt.count.view(torch.float32)[1:2]):
+        with pytest.raises(RuntimeError):
+            opt.run_optimizer(LR, grad_scale=scalar)
+        with pytest.raises(RuntimeError):
+            opt.run_optimizer(scalar)
+    with pytest.raises(RuntimeError):
+        grads.norm(out=g[:2])
+    assert opt.count.tolist() == [0, 0] and p.eq(1).all() and one.item() == 1 and g.eq(1).all()
+    opt.run_optimizer(g[:1], grad_scale=g[1:2])             # the step only reads gradients
+    assert opt.count.tolist() == [1, 0]
+
+
+def test_tensors_that_an_address_does_not_tell_are_refused():
+    sq = stochqn()
+    opt = sq.AdamW_free([torch.ones(300, device="cuda")])
+    i = torch.tensor([[3]], device="cuda")
+    for bad in (torch._neg_view(torch.ones(300, device="cuda")), torch.sparse_coo_tensor(i, torch.ones(1, device="cuda"), (300,)), None):
+        with pytest.raises(ValueError):
+            sq.TensorList([bad])
+        with pytest.raises(ValueError):
+            opt.update_gradient([bad])
+    opt.update_gradient([torch.ones(300, device="cuda")])
+    for bad in (torch._neg_view(torch.ones(300, device="cuda")), None):
+        with pytest.raises(ValueError):
+            opt.gradient.rebind([bad])
+    with pytest.raises(ValueError):
+        opt.run_optimizer(LR, grad_scale=torch._neg_view(torch.ones(1, device="cuda")))
+    assert opt.count.tolist() == [0, 0]
+
+
+def test_a_parameter_that_is_given_other_memory():
+    """The old memory stays until the optimizer goes, so nothing is written where others may be by now; the next gradient is refused."""
+    sq = stochqn()
+    p = torch.nn.Parameter(torch.ones(1000, device="cuda"))
+    opt = sq.AdamW_free([p], weight_decay=0.0)
+    g = torch.ones(1000, device="cuda")
+    opt.update_gradient([g])
+    p.data = torch.full((1000,), 7.0, device="cuda")
+    others = [torch.zeros(1000, device="cuda") for _ in range(50)]
+    opt.run_optimizer(LR)
+    torch.cuda.synchronize()
+    assert not any(o.any() for o in others) and p.eq(7).all()
+    with pytest.raises(ValueError):
+        opt.update_gradient([g])
+    with pytest.raises(ValueError):
+        opt.update_gradient(sq.TensorList([g]))
+    again = sq.AdamW_free([p], weight_decay=0.0)
+    again.load_state_dict(opt.state_dict())
+    again.update_gradient([g])
+    again.run_optimizer(LR)
+    assert again.count.tolist() == [2, 0] and p.lt(7).all()
+    grad = torch.ones(1000, device="cuda")                  # the same of a gradient: the list's memory stays
+    held = sq.TensorList([grad])
+    grad.data = torch.zeros(1, device="cuda")
+    others += [torch.zeros(1000, device="cuda") for _ in range(50)]
+    assert held.norm()[0].item() == pytest.approx(math.sqrt(1000), rel=torch.finfo(torch.float32).eps)
+
+
 def test_refusals():
     sq = stochqn()
     p = torch.zeros(300, device="cuda")
