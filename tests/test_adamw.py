@@ -1,6 +1,7 @@
 """The AdamW entries without a GPU: the reference's roundings against themselves, the C structure, refusals (nothing falls back to the CPU)."""
 import ctypes as C
 import os
+import re
 import subprocess
 
 import numpy as np
@@ -93,3 +94,61 @@ def test_the_host_side_under_sanitizers(which):
     for args in ([], ["threads"]) if which == "asan" else (["threads"],):
         run = subprocess.run([os.path.join(here, "build", "tensors_" + which)] + args, capture_output=True, text=True, timeout=300)
         assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr[-3000:]
+
+
+def kernels_of(asm):
+    """name -> basic blocks of every kernel of an assembly listing: (label or None, instructions, labels that may follow), in textual order; a block
+    that does not end in an unconditional jump or the program's end falls through to the next."""
+    found = {}
+    for name, body in re.findall(r"^(_Z\w+):.*?\n(.*?)^\.Lfunc_end", asm, re.M | re.S):
+        blocks = [[None, [], [], True]]
+        for line in body.splitlines():
+            line = line.split(";")[0].strip()
+            label = re.match(r"(\.LBB\w+):", line)
+            if label:
+                blocks.append([label.group(1), [], [], True])
+                continue
+            if not line or line.startswith("."):
+                continue
+            op = line.split()[0]
+            blocks[-1][1].append(line)
+            if op in ("s_branch", "s_endpgm") or op.startswith("s_cbranch"):
+                if op != "s_endpgm":
+                    blocks[-1][2].append(line.split()[1])
+                blocks[-1][3] = op.startswith("s_cbranch")
+                blocks.append([None, [], [], True])
+            elif op == "s_barrier":                                         # a block of its own end: what follows is behind it
+                blocks.append([None, [], [], True])
+            assert op not in ("s_setpc_b64", "s_swappc_b64"), line
+        found[name] = blocks
+    return found
+
+
+def reached(blocks, start, through):
+    at = {b[0]: k for k, b in enumerate(blocks) if b[0]}
+    seen, todo = set(), list(start)
+    while todo:
+        k = todo.pop()
+        if k in seen or k >= len(blocks):
+            continue
+        seen.add(k)
+        if through(blocks[k]):
+            todo += [at[label] for label in blocks[k][2]] + ([k + 1] if blocks[k][3] else [])
+    return seen
+
+
+def test_a_step_is_counted_behind_a_barrier(tmp_path):
+    """Every wave of a workgroup reads the step counter by itself, one thread arrives for all of them and the last to arrive writes it: in the
+    compiled kernels every way to an arrival, and to what is stored behind one, leads over a barrier of the workgroup."""
+    asm = tmp_path / "tensors.s"
+    subprocess.check_call(["make", "-C", os.path.join(ROOT, "stochqn_amd", "csrc"), "device-asm", "ASM=%s" % asm], stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
+    steps = {n: b for n, b in kernels_of(asm.read_text()).items() if "k_adamw" in n}
+    assert len(steps) == 6
+    for name, blocks in steps.items():
+        has = lambda b, what: any(line.startswith(what) for line in b[1])
+        arrivals = [k for k, b in enumerate(blocks) if has(b, "global_atomic")]
+        assert len(arrivals) == 2, name
+        counted = arrivals + [k for k in reached(blocks, arrivals, lambda b: True) if has(blocks[k], "global_store")]
+        assert len(counted) >= 5, name                                       # ... the stores that reset both counters, and the count
+        early = reached(blocks, [0], lambda b: not has(b, "s_barrier"))
+        assert not early & set(counted), name
