@@ -254,13 +254,16 @@ class AdamW_free:
         torch.autograd.graph.increment_version(self._versioned)          # a graph that saved the old weights cannot be run backward any more
 
     def _used_on(self, stream):
-        """... and its memory is not given to others before the work of those streams is done."""
-        self._on = stream
-        if stream not in self._streams and not torch.cuda.is_current_stream_capturing():
+        """... and its memory is not given to others before the work of those streams is done.  A capture runs nothing: the stream that it is made
+        on is still to be recorded at its first step outside of one."""
+        if stream not in self._streams:
+            if torch.cuda.is_current_stream_capturing():
+                return
             self._streams.add(stream)
             for t in (self.m, self.v, self.m_scale, self.v_scale, self.master, self.count, self._work):
                 if t is not None:
                     t.record_stream(torch.cuda.current_stream(self.params.device))
+        self._on = stream
 
     def __getstate__(self):
         raise TypeError("an AdamW_free holds a handle of the library: carry its state_dict() instead")

@@ -85,6 +85,51 @@ def test_the_words_are_uniform():
     assert (part == low[1000:1077]).all()
 
 
+class Recorded:
+    """Stands for an array of the state: which streams its memory was kept for."""
+
+    def __init__(self):
+        self.streams = []
+
+    def record_stream(self, stream):
+        self.streams.append(stream)
+
+
+def bare_optimizer(torch, **attributes):
+    """An AdamW_free without a GPU: its attributes are what is given, its library answers 0."""
+    class Library:
+        def stochqn_hip_adamw_step(self, *args):
+            return 0
+
+        def stochqn_hip_adamw_destroy(self, handle):
+            pass
+
+    class List:
+        device, _handle = torch.device("cuda", 0), 1
+
+    opt = object.__new__(adamw.AdamW_free)
+    opt.m, opt.v, opt.count, opt._work = (Recorded() for _ in range(4))
+    opt.m_scale = opt.v_scale = opt.master = None
+    opt._lib, opt._handle, opt.params, opt.gradient, opt._versioned, opt._on, opt._streams = Library(), 1, List(), List(), [], 10, {10}
+    for k, v in attributes.items():
+        setattr(opt, k, v)
+    return opt
+
+
+def test_a_stream_that_was_first_used_in_a_capture_is_recorded_at_its_first_eager_step(monkeypatch):
+    torch = pytest.importorskip("torch")
+    opt = bare_optimizer(torch)
+    now = {"stream": 10, "capturing": False}
+    monkeypatch.setattr(adamw, "_stream", lambda index: now["stream"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: now["stream"])
+    for stream, capturing, recorded in ((10, False, []), (20, True, []), (20, True, []), (20, False, [20]), (20, False, [20]), (10, False, [20]), (20, True, [20]),
+                                        (30, True, [20]), (20, False, [20]), (30, False, [20, 30]), (10, True, [20, 30]), (30, False, [20, 30])):
+        now.update(stream=stream, capturing=capturing)
+        opt.run_optimizer(0.1)
+        assert all(t.streams == recorded for t in (opt.m, opt.v, opt.count, opt._work)), (stream, capturing)
+
+
 @pytest.mark.parametrize("which", ["asan", "tsan"])
 def test_the_host_side_under_sanitizers(which):
     """What tensors.cpp hands to the kernels (every element of every tensor in one tile of one launch) and what it refuses, every HIP call failing

@@ -464,6 +464,34 @@ def test_the_state_outlives_the_work_of_every_stream_that_used_it():
     assert (w.double() - want).abs().max() <= 13 * 2.0 ** -24 * LR
 
 
+def test_the_state_outlives_a_stream_that_was_first_used_in_a_capture():
+    """As above, the second stream's first use a capture, whose work is not run: the eager step behind it is the one that must not outlive the memory."""
+    sq = stochqn()
+    n = 1 << 20
+    w, g = torch.zeros(n, device="cuda"), torch.ones(n, device="cuda")
+    big = torch.randn(4096, 4096, device="cuda")
+    opt = sq.AdamW_free([w])
+    opt.update_gradient([g])
+    size = opt.m.numel()
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        opt.run_optimizer(LR)
+    del graph                                               # (never replayed)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(200):
+            big = big @ big
+            big = big / big.abs().max()
+        opt.run_optimizer(LR)
+    del opt
+    fresh = [torch.full((size,), 7.0, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all((f == 7).all() for f in fresh)
+    want = -LR * 1.0 / (1.0 + 1e-8)
+    assert (w.double() - want).abs().max() <= 13 * 2.0 ** -24 * LR
+
+
 def test_copies_are_refused():
     import copy
     import pickle
