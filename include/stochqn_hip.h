@@ -282,7 +282,7 @@ size_t stochqn_hip_tensors_state(const stochqn_hip_tensors *tensors, size_t offs
 
 /* out[0] = |grad_scale| * sqrt(sum of all squares), out[1] = grad_scale * min(1, max_norm / out[0]): what the gradients are to be
  * multiplied with so that their norm, grad_scale (1 / loss scale) included, is at most max_norm (> 0; infinity: no clipping).  A norm
- * that is not finite makes out[1] NaN, which the step below takes as "reject".  Sums in f64, in an order that depends on the sizes
+ * that is not finite in f32 makes out[1] NaN, which the step below takes as "reject".  Sums in f64, in an order that depends on the sizes
  * alone.  work: stochqn_hip_tensors_norm_work() doubles that nothing else uses until the call's work is done.  With a communicator or
  * reducer installed the tensors are this rank's share and the sum is over all ranks (one double; every rank makes the call), like
  * every other sum of the library; work[0] holds it afterwards.  out, work and the tensors do not overlap.  Returns 0 or -1000. */

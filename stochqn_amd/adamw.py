@@ -131,7 +131,7 @@ class TensorList:
 
     def norm(self, max_norm=None, grad_scale=1.0, out=None):
         """A float32 tensor of two elements on the device: the norm over all tensors times `grad_scale` (1 / loss scale), and the factor
-        that brings the gradients to a norm of at most `max_norm` -- NaN if the norm is not finite, which makes the step that takes it
+        that brings the gradients to a norm of at most `max_norm` -- NaN if the norm is not finite as a float32, which makes the step that takes it
         (`run_optimizer(..., grad_scale=out[1:])`) a rejected one.  With a communicator installed: over all ranks' tensors."""
         max_norm = math.inf if max_norm is None else float(max_norm)
         if not max_norm > 0 or not math.isfinite(grad_scale):

@@ -488,13 +488,12 @@ template <int THREADS> __device__ inline double block_sum(double x)
 	return x;
 }
 
-// a norm that is not finite leaves NaN as the coefficient: the step that takes it is rejected
+// A norm that is not finite leaves NaN as the coefficient: the step that takes it is rejected.  Finite is what the caller sees, in f32.
 __device__ inline void verdict(double sum, double grad_scale, double max_norm, float* out)
 {
 	const double norm = sqrt(sum) * fabs(grad_scale);
-	const bool finite = norm <= 1.7976931348623157e308;
 	out[0] = (float) norm;
-	out[1] = !finite ? __builtin_nanf("") : (float) (norm > max_norm ? grad_scale * (max_norm / norm) : grad_scale);
+	out[1] = !__builtin_isfinite((float) norm) ? __builtin_nanf("") : (float) (norm > max_norm ? grad_scale * (max_norm / norm) : grad_scale);
 }
 
 template <int TILE, Kind K> __device__ inline double squares(const void* grad, uint64_t first, uint64_t n, int type, double sum)

@@ -343,6 +343,30 @@ def test_norm_of_what_is_not_finite_zero_and_huge():
             assert not math.isfinite(float(out[0])) and math.isnan(float(out[1]))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [5, 100_000])
+def test_norm_at_the_end_of_the_range(dtype, n):
+    """The norm that the caller sees is f32: past its range it is infinite, and the coefficient says so too, though the sum in f64 is finite."""
+    g = torch.zeros(n, dtype=dtype, device="cuda")
+    grads = stochqn().TensorList([g])
+    g[n // 2] = 3e38
+    x = float(g[n // 2])
+    for max_norm in (None, 1.0):
+        out = grads.norm(max_norm=max_norm).tolist()
+        assert out[0] == np.float32(x) and out[1] == (1.0 if max_norm is None else np.float32(1.0 / x))
+    g[0] = 3e38                                             # the norm is 4.2e38
+    for max_norm in (None, 1.0, 1e300):
+        out = grads.norm(max_norm=max_norm).tolist()
+        assert out[0] == math.inf and math.isnan(out[1])
+    for scale, ok in ((0.5, True), (-0.5, True), (2.0, False), (1e-300, True)):
+        out = grads.norm(max_norm=1e-3, grad_scale=scale).tolist()
+        want = abs(scale) * math.sqrt(2.0) * x
+        assert math.isfinite(out[0]) == math.isfinite(out[1]) == ok, scale
+        # one rounding of each to f32, or half its least subnormal, beside the f64 ones
+        coef = scale * min(1.0, 1e-3 / want)
+        assert not ok or (abs(out[0] - want) <= 1.001 * 2.0 ** -24 * want + 2.0 ** -150 and abs(out[1] - coef) <= 1.001 * 2.0 ** -24 * abs(coef) + 2.0 ** -150)
+
+
 def test_a_clipped_step_with_a_loss_scale_and_a_schedule():
     """norm -> step, the coefficient never on the host: as a training loop would, four steps, one of them with an overflowed gradient."""
     model = Model([4000, 129, 1000], F16, F16, seed=8, grad_size=30.0)
