@@ -309,7 +309,7 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors *tensors, double grad_scale, do
  * step_size_dev or grad_scale with one.
  * step:  grads: as many tensors, of the same sizes, f32 / bf16 / f16 each; step_size_dev (nullable): a float on the device in place of
  * step_size (schedules in a captured graph); grad_scale (nullable = 1): a float on the device, out + 1 of the norm.  If either
- * is not finite the step is rejected: nothing is written and nothing counted -- the guard of take_step, left on the device.  Returns 0 or
+ * is not finite, or step_size / (1 - beta1^t) or 1 - step_size weight_decay is not in f32, the step is rejected: nothing is written and nothing counted -- the guard of take_step, left on the device.  Returns 0 or
  * -1000. */
 typedef struct stochqn_hip_adamw_setup {
 	double beta1, beta2, eps, weight_decay;

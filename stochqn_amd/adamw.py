@@ -235,8 +235,8 @@ class AdamW_free:
 
     def run_optimizer(self, step_size, grad_scale=None):
         """One step.  step_size: a number, or a float32 tensor of one element on the device (schedules in a captured graph).  grad_scale: None,
-        or such a tensor that every gradient is multiplied with (`TensorList.norm(...)[1:]`).  If either is not finite the step is
-        rejected: no weight, no moment and no count changes."""
+        or such a tensor that every gradient is multiplied with (`TensorList.norm(...)[1:]`).  If either is not finite (or
+        step_size / (1 - beta1 ** t), or step_size * weight_decay, is past float32) the step is rejected: no weight, no moment and no count changes."""
         if self.gradient is None:
             raise ValueError("no gradient: call update_gradient first.")
         dev = self.params.device

@@ -171,7 +171,8 @@ struct Step {
 __device__ inline Step step_of(const AdamwArgs& a, long long t, float scale, double lr)
 {
 	Step s{};
-	// a scale or a step size that is not finite: the step is rejected as a whole, nothing changes and nothing is counted
+	// A scale or a step size that is not finite, here or as the f32 numbers formed below: the step is rejected as a whole, nothing changes and
+	// nothing is counted.  Every wave of every launch of the step decides alike: by the same scalars and the same count.
 	s.scale = scale;
 	s.go = __builtin_isfinite(s.scale) && __builtin_isfinite(lr);
 	if (!s.go) return s;
@@ -194,6 +195,7 @@ __device__ inline Step step_of(const AdamwArgs& a, long long t, float scale, dou
 	y1 = fma(fma(-d1, y1, 1.0), y1, y1);
 	y2 = fma(fma(-d2 * y2, y2, 1.0), 0.5 * y2, y2);
 	s.rate = (float) (lr * y1);
+	s.go = __builtin_isfinite(s.rate) && __builtin_isfinite(s.decay);
 	s.root = (float) y2;
 	s.eps = a.eps;
 	s.key = finalise(a.seed ^ (uint64_t) t * kStepKey);

@@ -197,6 +197,24 @@ def test_a_scale_from_the_device_and_a_rejected_step(bits):
     check_step(model, opt, grad_scale=scale)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_whose_numbers_are_past_f32_is_rejected(bits):
+    """A step size that is finite, but not as the f32 numbers that the step is taken with: step_size / (1 - beta1^t) and 1 - step_size * weight_decay."""
+    model = Model([1000, 77], F32, F32, seed=5)
+    for decay, rates in ((0.0, (1e39, -1e39, 1e300, 3.5e37, -3.5e37, torch.tensor(3.5e37, device="cuda"))), (1e30, (1e9, -1e9, torch.tensor(1e9, device="cuda")))):
+        opt = stochqn().AdamW_free(model.params, state_bits=bits, weight_decay=decay)
+        opt.update_gradient(model.grads)
+        kept = [opt.m, opt.v, opt.count] + model.params + ([opt.m_scale, opt.v_scale] if bits == 8 else [])
+        was = [t.view(torch.uint8).clone() for t in kept]
+        for rate in rates:
+            opt.run_optimizer(rate)
+            assert all((t.view(torch.uint8) == w).all() for t, w in zip(kept, was)), rate
+        opt.run_optimizer(3.3e37 if not decay else 3.3e8)   # (divided by 0.1, times 1e30: 3.3e38, within f32)
+        assert opt.count.tolist() == [1, 0]
+        for p in model.params:
+            p.zero_()
+
+
 def test_eight_bit_blocks_with_nothing_tiny_huge_and_not_finite():
     n = 128 * 12 + 40
     model = Model([n], F32, F32, seed=1)
