@@ -305,7 +305,7 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors *tensors, double grad_scale, do
  *   decay             one byte per tensor, 0: no weight decay for it; NULL: all decay
  *   count             two int64: steps taken; zero (arrivals within a step)
  *   work              4096 bytes, aligned to 8, zero: arrivals as well
- * m, v, master aligned to 16 bytes.  eps >= 2^-126.  No two arrays that the step writes may overlap, nor a gradient,
+ * m, v, master aligned to 16 bytes.  2^-126 <= eps <= 2^126.  No two arrays that the step writes may overlap, nor a gradient,
  * step_size_dev or grad_scale with one.
  * step:  grads: as many tensors, of the same sizes, f32 / bf16 / f16 each; step_size_dev (nullable): a float on the device in place of
  * step_size (schedules in a captured graph); grad_scale (nullable = 1): a float on the device, out + 1 of the norm.  If either

@@ -167,7 +167,7 @@ class AdamW_free:
     def __init__(self, params, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, state_bits=32, master=False, stochastic=False,
                  decay=None, seed=0):
         assert 0 <= beta1 < 1 and 0 <= beta2 < 1
-        assert 2.0 ** -126 <= eps < 3e38 and math.isfinite(weight_decay)
+        assert 2.0 ** -126 <= eps <= 2.0 ** 126 and math.isfinite(weight_decay)
         assert state_bits in (8, 32)
         assert not (master and stochastic)
         self.params = params if isinstance(params, TensorList) else TensorList(params)

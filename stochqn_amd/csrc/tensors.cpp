@@ -317,7 +317,7 @@ stochqn_hip_adamw* stochqn_hip_adamw_create(stochqn_hip_tensors* params, const s
 		if (!params || !setup) refuse("an argument is NULL");
 		const stochqn_hip_adamw_setup& s = *setup;
 		if (!(s.beta1 >= 0 && s.beta1 < 1) || !(s.beta2 >= 0 && s.beta2 < 1)) refuse("beta1 and beta2 lie in [0, 1)");
-		if (!(s.eps >= FLT_MIN && s.eps <= FLT_MAX)) refuse("eps has to be a positive number of 32 bits");
+		if (!(s.eps >= FLT_MIN && s.eps <= 1 / FLT_MIN)) refuse("eps lies in 2^-126 .. 2^126");       // sqrt(v) adds nothing to the largest, whose reciprocal is not subnormal
 		if (!std::isfinite(s.weight_decay)) refuse("weight_decay is not finite");
 		if (s.state_bits != 32 && s.state_bits != 8) refuse("state_bits is 32 or 8");
 		if (s.state_bits == 32 && (s.m_scale || s.v_scale)) refuse("moments in 32 bits have no scales");

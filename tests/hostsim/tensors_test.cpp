@@ -237,6 +237,7 @@ static void refusals()
 	CHECK(refused([](auto& s) { s.m = nullptr; }) && refused([](auto& s) { s.count = nullptr; }) && refused([](auto& s) { s.work = nullptr; }));
 	CHECK(refused([](auto& s) { s.v = s.m; }) && refused([](auto& s) { s.m = (char*) s.m + 4; }) && refused([&](auto& s) { s.master = (float*) l.p[0]; }));
 	CHECK(refused([](auto& s) { s.m = device_block(16); }) && refused([](auto& s) { s.m = device_block(1 << 16, 1); }) && refused([](auto& s) { s.stochastic = 1; }));
+	CHECK(!refused([](auto& s) { s.eps = 0x1p126; }) && refused([](auto& s) { s.eps = 0x1.000002p126; }) && refused([](auto& s) { s.eps = 3e38; }));      // its reciprocal is subnormal
 	stochqn_hip_adamw* o = stochqn_hip_adamw_create(l.params, &good);
 	CHECK(o);
 	g_launches.clear();

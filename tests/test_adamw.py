@@ -45,6 +45,13 @@ def test_no_gpu_or_no_device_memory_is_refused(capfd):
     assert "stochqn_hip_adamw_step: an argument is NULL" in err
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-39, 2.0 ** 126 * (1 + 2.0 ** -23), 2e38, float("inf"), float("nan")])
+def test_an_eps_that_the_step_cannot_divide_by_is_refused(eps):
+    torch = pytest.importorskip("torch")
+    with pytest.raises(AssertionError):
+        stochqn_amd.AdamW_free([torch.zeros(3)], eps=eps)
+
+
 @pytest.mark.parametrize("which", ["m", "v"])
 def test_the_reference_rounds_to_a_neighbour_and_keeps_the_mean(which):
     """encode then decode: within one step of the code, exact for what the format holds, the mean of many words the value itself."""

@@ -288,6 +288,20 @@ def test_tiny_gradients_beside_a_tiny_eps(bits):
     assert (np.abs(host(w) - want)[sure] <= ((0.6 * off + 10 * 2.0 ** -24) * np.abs(want))[sure]).all()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_largest_eps(bits):
+    """eps = 2^126, whose reciprocal is the least normal number: the update against the formula; a larger one is refused (its reciprocal is among the
+    subnormals, which the hardware's takes for zero)."""
+    model = Model([300], F32, F32, grad_size=1e18)
+    model.params[0].zero_()
+    opt = stochqn().AdamW_free(model.params, eps=2.0 ** 126, weight_decay=0.0, state_bits=bits)
+    opt.update_gradient(model.grads)
+    check_step(model, opt, lr=1e30)
+    assert model.params[0].abs().max() > 1e6
+    with pytest.raises(AssertionError):
+        stochqn().AdamW_free(model.params, eps=2.0 ** 126 * (1 + 2.0 ** -23))
+
+
 def test_autograd_knows_that_the_weights_were_written():
     w = torch.randn(100, device="cuda", requires_grad=True)
     x = torch.ones(100, device="cuda")
