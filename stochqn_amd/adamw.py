@@ -216,7 +216,11 @@ class AdamW_free:
 
     def update_gradient(self, gradient):
         """Name the gradients of the coming steps: tensors (or a TensorList) in the order of the parameters.  Nothing is copied: the steps
-        read what the tensors hold by then.  The parameters have to be where they were when the object was made (no `.data = ...`)."""
+        read what the tensors hold by then, and they are held until others are named.  None lets go of them, so that a backward pass which makes
+        new ones does not find the old ones beside it.  The parameters have to be where they were when the object was made (no `.data = ...`)."""
+        if gradient is None:
+            self.gradient, self._own_list = None, False
+            return
         if [t.data_ptr() for t in self.tensors] != self._at:
             raise ValueError("a parameter has other memory than when the optimizer was made: make a new one, with the old one's state.")
         if isinstance(gradient, TensorList):
@@ -225,7 +229,7 @@ class AdamW_free:
             self.gradient, self._own_list = gradient, False
             return
         gradient = list(gradient)
-        if self._own_list and [getattr(t, "dtype", None) for t in gradient] == self.gradient.dtypes:
+        if self._own_list and self.gradient is not None and [getattr(t, "dtype", None) for t in gradient] == self.gradient.dtypes:
             self.gradient.rebind(gradient)
             return
         new = TensorList(gradient)

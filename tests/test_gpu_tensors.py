@@ -726,6 +726,38 @@ def test_a_parameter_that_is_given_other_memory():
     assert held.norm()[0].item() == pytest.approx(math.sqrt(1000), rel=torch.finfo(torch.float32).eps)
 
 
+def test_gradients_are_let_go():
+    """Between two steps nothing of the last gradients has to stay: their memory is free for the next backward pass."""
+    sq = stochqn()
+    n = 1 << 20
+    p = torch.nn.Parameter(torch.ones(n, device="cuda"))
+    opt = sq.AdamW_free([p])
+    held = []
+    for how in ("update_gradient", "attribute", "update_gradient"):
+        before = torch.cuda.memory_allocated()
+        (p * p).sum().backward()
+        opt.update_gradient([p.grad])
+        opt.run_optimizer(LR)
+        p.grad = None
+        held.append(torch.cuda.memory_allocated() - before)
+        if how == "attribute":
+            opt.gradient = None
+        else:
+            opt.update_gradient(None)
+        assert torch.cuda.memory_allocated() == before, how
+        assert opt.gradient is None
+        with pytest.raises(ValueError):
+            opt.run_optimizer(LR)
+    assert min(held) >= 4 * n and opt.count.tolist() == [3, 0]
+    mine = sq.TensorList([torch.ones(n, device="cuda")])    # a list of the caller's is the caller's to drop
+    opt.update_gradient(mine)
+    opt.update_gradient(None)
+    assert abs(float(mine.norm()[0]) - 1024) <= 2.0 ** -24 * 1024
+    opt.update_gradient([torch.ones(n, device="cuda")])
+    opt.run_optimizer(LR)
+    assert opt.count.tolist() == [4, 0] and mine.tensors[0].eq(1).all()
+
+
 def test_refusals():
     sq = stochqn()
     p = torch.zeros(300, device="cuda")
