@@ -726,6 +726,32 @@ def test_a_parameter_that_is_given_other_memory():
     assert held.norm()[0].item() == pytest.approx(math.sqrt(1000), rel=torch.finfo(torch.float32).eps)
 
 
+def test_the_training_loop_of_the_documentation():
+    """The loop as it is printed there, run on three batches: the weights and moments of a loop that takes each batch's own gradients."""
+    import os
+    import re
+    sq = stochqn()
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")).read()
+    code = re.search(r"## Models of many tensors.*?```python\n(.*?)```", text, re.S).group(1)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    first = [torch.randn(64, 40, generator=gen, device="cuda").half(), torch.randn(40, generator=gen, device="cuda").half()]
+    data = [torch.randn(8, 64, generator=gen, device="cuda").half() for _ in range(3)]
+    params = [torch.nn.Parameter(p.clone()) for p in first]
+    loss = lambda batch, p=None: ((batch @ (p or params)[0] + (p or params)[1]).float() ** 2).mean()
+    names = dict(params=params, data=data, loss=loss, lr=LR)
+    exec(code, names)
+    mine = [p.clone() for p in first]
+    opt = sq.AdamW_free(mine, weight_decay=0.1, state_bits=8, master=True, decay=[p.ndim > 1 for p in mine])
+    for batch in data:
+        leaves = [p.detach().clone().requires_grad_() for p in mine]
+        grads = sq.TensorList(torch.autograd.grad(loss(batch, leaves) * 1024, leaves))
+        opt.update_gradient(grads)
+        opt.run_optimizer(LR, grad_scale=grads.norm(max_norm=1.0, grad_scale=1 / 1024)[1:])
+    assert names["opt"].count.tolist() == [3, 0] and all(p.ne(q).any() for p, q in zip(params, first))
+    for a, b in zip(params + [names["opt"].m, names["opt"].v, names["opt"].master], mine + [opt.m, opt.v, opt.master]):
+        assert (a.detach().view(torch.uint8) == b.view(torch.uint8)).all()
+
+
 def test_gradients_are_let_go():
     """Between two steps nothing of the last gradients has to stay: their memory is free for the next backward pass."""
     sq = stochqn()
