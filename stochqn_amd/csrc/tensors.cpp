@@ -263,7 +263,7 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors* t, double grad_scale, double m
 		if (!t || !out || !work) refuse("an argument is NULL");
 		if (!std::isfinite(grad_scale)) refuse("grad_scale is not finite");
 		if (!(max_norm > 0)) refuse("max_norm is not positive");
-		std::lock_guard<std::mutex> lk(t->mu);
+		std::unique_lock<std::mutex> lk(t->mu);
 		int device = t->device;
 		check_aligned(out, sizeof(float), "out");
 		check_aligned(work, sizeof(double), "work");
@@ -302,6 +302,7 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors* t, double grad_scale, double m
 				parts += grid;
 				launches++;
 			});
+		lk.unlock();                                                // the launches have the addresses; a reducer may wait for a thread that wants this list
 		if (!done) launch_norm_sum(st, work, parts, grad_scale, max_norm, reduced ? nullptr : out);
 		if (reduced) {
 			if (!reduce_in_place(work, 1, st)) refuse("the reduction over the ranks failed");

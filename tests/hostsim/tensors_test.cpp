@@ -4,6 +4,8 @@
 #include "runtime.hpp"
 #include "stochqn_hip.h"
 
+#include <atomic>
+#include <chrono>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -66,6 +68,8 @@ struct Launch { char kind; int bits, tile, grid, on; hipStream_t st; sqn::Table<
 static std::vector<Launch> g_launches;
 static int g_ranks = 1;
 static bool g_fail_launch = false, g_fail_reduce = false;
+static std::atomic<bool> g_meeting{false};
+static std::atomic<int> g_arrived{0};
 static std::mutex g_mu;
 static void launched_one(Launch l) { std::lock_guard<std::mutex> lk(g_mu); l.on = g_device; g_launches.push_back(l); if (g_fail_launch) g_launch_error = hipErrorLaunchFailure; }
 namespace sqn {
@@ -75,7 +79,15 @@ void launch_norm_sum(hipStream_t st, double*, int count, double, double, float* 
 void launch_norm_verdict(hipStream_t st, const double*, double, double, float* out) { Launch l{}; l.kind = 'v'; l.st = st; l.out = out; launched_one(l); }
 bool device_ready() { return true; }
 int comm_nranks() { return g_ranks; }
-bool reduce_in_place(double*, int, hipStream_t) { return !g_fail_reduce; }
+bool reduce_in_place(double*, int, hipStream_t)
+{
+	if (g_meeting.load()) {                                                     // a reducer that returns when both ranks are there, or gives up
+		const int mine = ++g_arrived;
+		for (int k = 0; k < 5000 && g_arrived.load() < (mine + 1) / 2 * 2; k++) std::this_thread::sleep_for(std::chrono::milliseconds(1));
+		return g_arrived.load() >= (mine + 1) / 2 * 2;
+	}
+	return !g_fail_reduce;
+}
 }
 
 #define CHECK(x) do { if (!(x)) { std::printf("FAILED line %d: %s\n", __LINE__, #x); std::exit(1); } } while (0)
@@ -381,9 +393,27 @@ static void concurrent()
 	stochqn_hip_adamw_destroy(q);
 }
 
+// Two ranks of one process that take the norm of one list at once: a list must not be held while its rank waits for the other.
+static void two_ranks_of_one_list()
+{
+	Lists l({3000, 40});
+	const size_t bytes = 8 * stochqn_hip_tensors_norm_work(l.grads);
+	g_ranks = 2;
+	g_meeting = true;
+	const auto rank = [&](float* out, double* work) { for (int k = 0; k < 3; k++) CHECK(stochqn_hip_tensors_norm(l.grads, 1, 1, out, work, nullptr) == 0); };
+	float *one = (float*) device_block(8), *two = (float*) device_block(8);
+	double *w1 = (double*) device_block(bytes), *w2 = (double*) device_block(bytes);
+	std::thread a([&] { rank(one, w1); }), b([&] { rank(two, w2); });
+	a.join();
+	b.join();
+	CHECK(g_arrived == 6);
+	g_ranks = 1;
+	g_meeting = false;
+}
+
 int main(int argc, char**)
 {
-	if (argc > 1) { concurrent(); std::printf("ok\n"); return 0; }
+	if (argc > 1) { concurrent(); two_ranks_of_one_list(); std::printf("ok\n"); return 0; }
 	for (int bits : {32, 8}) {
 		covers({}, bits, 0);
 		covers({0, 0, 0}, bits, 0);
