@@ -264,7 +264,7 @@ int stochqn_hip_comm_allreduce_probe(int count, int reps, double *median_us, dou
  * the quasi-Newton steps above, which take one flat vector.  Independent of real_t: a tensor is f32, bf16 or f16 in either build.
  * Everything is device memory of one device; the calls work on the stream they are given (a hipStream_t of that device, NULL = its
  * NULL stream), in order with it, whichever device is current; they allocate nothing, copy nothing, do not synchronise and may be
- * captured into a graph.  They have no context, so the built-in profiler does not see them.
+ * captured into a graph (the norm over several ranks: as its reducer does).  They have no context, so the built-in profiler does not see them.
  * A list names tensors: contiguous, aligned to their element size, of any length (0 included: the address is not looked at).  The
  * state of a parameter of k elements starts at a multiple of 128 elements and takes the next multiple of 128 from k on.
  * Handles may be used by several threads at once; calls that write the same arrays have to be ordered by their caller, by stream. */
@@ -285,7 +285,10 @@ size_t stochqn_hip_tensors_state(const stochqn_hip_tensors *tensors, size_t offs
  * that is not finite in f32 makes out[1] NaN, which the step below takes as "reject".  Sums in f64, in an order that depends on the sizes
  * alone.  work: stochqn_hip_tensors_norm_work() doubles that nothing else uses until the call's work is done.  With a communicator or
  * reducer installed the tensors are this rank's share and the sum is over all ranks (one double; every rank makes the call), like
- * every other sum of the library; work[0] holds it afterwards.  out, work and the tensors do not overlap.  Returns 0 or -1000. */
+ * every other sum of the library; work[0] holds it afterwards.  RCCL's sum is enqueued like the rest: the call does not wait for the other
+ * ranks, so a rank whose peer never comes finds out in a wait of its own, which "reducer_patience_s" does not bound.  A reducer of the caller's
+ * runs within the call, and synchronises, and may be captured, as far as it does; the loop-back reducer synchronises (bounded) and its sums are
+ * refused in a capture.  out, work and the tensors do not overlap.  Returns 0 or -1000. */
 size_t stochqn_hip_tensors_norm_work(const stochqn_hip_tensors *tensors);
 int stochqn_hip_tensors_norm(stochqn_hip_tensors *tensors, double grad_scale, double max_norm, float out[], double work[], void *hip_stream);
 

@@ -1358,6 +1358,8 @@ bool reduce_in_place(double* buf, int count, hipStream_t st)
 	return !c.fault && !failed;
 }
 
+bool reduces_on_the_host() { return current_reducer().kind == Reducer::LOOP; }
+
 int comm_nranks()
 {
 	const Reducer r = current_reducer();

@@ -307,6 +307,7 @@ int comm_nranks();
 void comm_attach(DevCtx* c);                           // install the all-reduce hook, compute n_global
 Reducer current_reducer();                             // the calling thread's binding, else the process-wide communicator
 bool reduce_in_place(double* buf, int count, hipStream_t st);   // sum over the ranks of the calling thread's reducer, on the caller's stream (calls without a context)
+bool reduces_on_the_host();                            // that reducer waits for the stream and sums host copies: its sums cannot be captured into a graph
 void set_thread_reducer(const Reducer& r);             // contexts created by this thread from now on reduce through `r`
 bool comm_init_all(int ndev, const int* devices, void** comms_out);   // ncclCommInitAll (one process, ndev devices)
 void comm_destroy(void* comm);

@@ -278,8 +278,12 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors* t, double grad_scale, double m
 		}
 		OnDevice on(device);
 		hipStream_t st = check_stream(hip_stream, device);
-		(void) hipGetLastError();                                  // somebody else's: only what the launches below leave counts
 		const bool reduced = comm_nranks() > 1;
+		if (reduced && reduces_on_the_host()) {
+			hipStreamCaptureStatus capture;
+			if (hipStreamIsCapturing(st, &capture) != hipSuccess || capture != hipStreamCaptureStatusNone) refuse("the ranks' sums are formed on the host: they cannot be captured");
+		}
+		(void) hipGetLastError();                                  // somebody else's: only what the launches below leave counts
 		Table<NormArgs, kEntries> table;
 		NormArgs& a = table.a;
 		a.grad_scale = grad_scale;

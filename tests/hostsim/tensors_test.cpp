@@ -18,6 +18,7 @@ struct Block { uintptr_t at; size_t bytes; int device; };
 static std::vector<Block> g_blocks;
 static thread_local int g_device = 0, g_launch_error = 0;
 static int g_fail_after = -1;
+static bool g_capturing = false;
 static uintptr_t g_next = (uintptr_t) 1 << 40;       // far below what the process itself uses
 
 static void* device_block(size_t bytes, int device = 0, size_t shift = 0)
@@ -58,6 +59,7 @@ hipError_t hipMemGetAddressRange(hipDeviceptr_t* base, size_t* size, hipDevicept
 hipError_t hipGetDevice(int* d) { if (failing()) return hipErrorUnknown; *d = g_device; return hipSuccess; }
 hipError_t hipSetDevice(int d) { if (failing()) return hipErrorUnknown; g_device = d; return hipSuccess; }
 hipError_t hipStreamGetDevice(hipStream_t s, hipDevice_t* d) { if (failing()) return hipErrorUnknown; *d = (int) ((uintptr_t) s >> 8); return hipSuccess; }
+hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus* s) { if (failing()) return hipErrorUnknown; *s = g_capturing ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone; return hipSuccess; }
 hipError_t hipDeviceGetAttribute(int* v, hipDeviceAttribute_t, int) { if (failing()) return hipErrorUnknown; *v = 256; return hipSuccess; }
 hipError_t hipGetLastError() { const int e = g_launch_error; g_launch_error = 0; return (hipError_t) e; }
 const char* hipGetErrorString(hipError_t) { return "an error"; }
@@ -67,7 +69,7 @@ const char* hipGetErrorString(hipError_t) { return "an error"; }
 struct Launch { char kind; int bits, tile, grid, on; hipStream_t st; sqn::Table<sqn::AdamwArgs, sqn::kEntries> a; sqn::Table<sqn::NormArgs, sqn::kEntries> n; int count; bool out; };
 static std::vector<Launch> g_launches;
 static int g_ranks = 1;
-static bool g_fail_launch = false, g_fail_reduce = false;
+static bool g_fail_launch = false, g_fail_reduce = false, g_on_the_host = false;
 static std::atomic<bool> g_meeting{false};
 static std::atomic<int> g_arrived{0};
 static std::mutex g_mu;
@@ -79,6 +81,7 @@ void launch_norm_sum(hipStream_t st, double*, int count, double, double, float* 
 void launch_norm_verdict(hipStream_t st, const double*, double, double, float* out) { Launch l{}; l.kind = 'v'; l.st = st; l.out = out; launched_one(l); }
 bool device_ready() { return true; }
 int comm_nranks() { return g_ranks; }
+bool reduces_on_the_host() { return g_on_the_host; }
 bool reduce_in_place(double*, int, hipStream_t)
 {
 	if (g_meeting.load()) {                                                     // a reducer that returns when both ranks are there, or gives up
@@ -298,6 +301,21 @@ static void refusals()
 	g_ranks = 2;
 	g_fail_reduce = true;
 	CHECK(stochqn_hip_tensors_norm(l.grads, 1, 1, out, work, nullptr) == -1000);
+	g_fail_reduce = false;
+	// a sum that the host forms is not captured: refused in front of the first launch; any other call goes on
+	for (bool capturing : {false, true})
+		for (bool host_side : {false, true})
+			for (int ranks : {1, 2}) {
+				g_capturing = capturing;
+				g_on_the_host = host_side;
+				g_ranks = ranks;
+				g_launches.clear();
+				const int rc = stochqn_hip_tensors_norm(l.grads, 1, 1, out, work, nullptr);
+				const bool no = capturing && host_side && ranks == 2;
+				CHECK(rc == (no ? -1000 : 0) && g_launches.empty() == no);
+				CHECK(stochqn_hip_adamw_step(o, l.grads, 0.1, nullptr, nullptr, nullptr) == 0);
+			}
+	g_capturing = g_on_the_host = false;
 	g_ranks = 1;
 	// another current device: the launches go to the tensors', and the caller's is current again
 	{

@@ -908,3 +908,33 @@ def test_the_norm_over_the_ranks_of_a_reducer():
         lib.stochqn_hip_loopback_finalize()
     assert out[0] == out[1]
     assert abs(out[0][0] - want) <= 2.0 ** -23 * want and abs(out[0][1] * want - 1) <= 2.0 ** -23
+
+
+def test_the_norm_over_a_host_side_reducer_is_refused_in_a_capture():
+    """The refused call leaves the capture as it was: what else is captured is replayed."""
+    sq = stochqn()
+    lib = sq.cdll()
+    g = torch.full((1000,), 2.0, device="cuda")
+    grads, x, out = sq.TensorList([g]), torch.zeros(5, device="cuda"), []
+    assert lib.stochqn_hip_loopback_init(2) == 0
+    try:
+        def work():
+            assert lib.stochqn_hip_loopback_join(0) == 0
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                x.add_(1)
+                try:
+                    grads.norm()
+                except RuntimeError as e:
+                    out.append(e)
+                x.add_(1)
+            graph.replay()
+            graph.replay()
+            torch.cuda.synchronize()
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+    finally:
+        lib.stochqn_hip_loopback_finalize()
+    assert len(out) == 1 and x.eq(4).all()
+    assert abs(float(grads.norm()[0]) - 2 * math.sqrt(1000)) <= 2.0 ** -23 * 64     # this thread has no reducer
