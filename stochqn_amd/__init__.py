@@ -64,7 +64,18 @@ def lib(use_float=False):
 
 from .free import oLBFGS_free, SQN_free, adaQN_free  # noqa: E402
 
-__all__ = ["lib", "cdll", "LIB_PATH", "oLBFGS_free", "SQN_free", "adaQN_free", "AdamW_free", "TensorList"]
+__all__ = ["lib", "cdll", "LIB_PATH", "oLBFGS_free", "SQN_free", "adaQN_free"]
+
+
+def _has_torch():
+    try:
+        return "torch" in _sys.modules or _ilu.find_spec("torch") is not None
+    except (ImportError, ValueError):
+        return False
+
+
+if _has_torch():                # a star import looks every name up: without torch these two would end it
+    __all__ += ["AdamW_free", "TensorList"]
 
 
 def __getattr__(name):

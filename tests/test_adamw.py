@@ -3,6 +3,7 @@ import ctypes as C
 import os
 import re
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -22,6 +23,23 @@ def test_the_setup_structure_is_the_header_s(tmp_path):
     subprocess.check_call(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "t")])
     got = [int(x) for x in subprocess.check_output([str(tmp_path / "t")]).split()]
     assert got == [C.sizeof(adamw._Setup)] + [getattr(adamw._Setup, n).offset for n in names]
+
+
+@pytest.mark.parametrize("torch_is_there", [False, True])
+def test_a_star_import_needs_no_torch(torch_is_there):
+    """The free-mode objects do without torch, under every import; the objects over tensors come with it."""
+    code = ("import sys\n"
+            "class No:\n"
+            "    def find_spec(self, name, path=None, target=None):\n"
+            "        if name.split('.')[0] == 'torch':\n"
+            "            raise ModuleNotFoundError(name)\n"
+            "    def invalidate_caches(self):\n"
+            "        pass\n"
+            "%s"
+            "from stochqn_amd import *\n"
+            "assert oLBFGS_free and SQN_free and adaQN_free and lib and cdll\n"
+            "assert ('AdamW_free' in globals()) == ('TensorList' in globals()) == %s\n")
+    subprocess.check_call([sys.executable, "-c", code % ("" if torch_is_there else "sys.meta_path.insert(0, No())\n", torch_is_there)], cwd=ROOT)
 
 
 def test_no_gpu_or_no_device_memory_is_refused(capfd):
