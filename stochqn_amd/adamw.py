@@ -241,7 +241,8 @@ class AdamW_free:
         """One step.  step_size: a number, or a float32 tensor of one element on the device (schedules in a captured graph).  grad_scale: None,
         or such a tensor that every gradient is multiplied with (`TensorList.norm(...)[1:]`).  If either is not finite (or
         step_size / (1 - beta1 ** t), or step_size * weight_decay, is past float32) the step is rejected: no weight, no moment and no count changes."""
-        if self.gradient is None:
+        gradient = self.gradient                        # this step's, also if another thread names others meanwhile
+        if gradient is None:
             raise ValueError("no gradient: call update_gradient first.")
         dev = self.params.device
         step_dev = None
@@ -253,7 +254,7 @@ class AdamW_free:
         stream = _stream(dev.index)
         if stream != self._on:
             self._used_on(stream)
-        if self._lib.stochqn_hip_adamw_step(self._handle, self.gradient._handle, step_size, step_dev, scale, stream) != 0:
+        if self._lib.stochqn_hip_adamw_step(self._handle, gradient._handle, step_size, step_dev, scale, stream) != 0:
             raise RuntimeError("stochqn_hip_adamw_step failed (its reason is on stderr).")
         torch.autograd.graph.increment_version(self._versioned)          # a graph that saved the old weights cannot be run backward any more
 

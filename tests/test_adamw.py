@@ -4,6 +4,7 @@ import os
 import re
 import subprocess
 import sys
+import weakref
 
 import numpy as np
 import pytest
@@ -153,6 +154,25 @@ def test_a_stream_that_was_first_used_in_a_capture_is_recorded_at_its_first_eage
         now.update(stream=stream, capturing=capturing)
         opt.run_optimizer(0.1)
         assert all(t.streams == recorded for t in (opt.m, opt.v, opt.count, opt._work)), (stream, capturing)
+
+
+def test_the_gradients_live_as_long_as_the_step_that_reads_them():
+    """Another thread names other gradients while a step is in the library, which has let go of Python's lock: the list that the step was given stays."""
+    torch = pytest.importorskip("torch")
+    opt = bare_optimizer(torch)
+    alive = weakref.ref(opt.gradient)
+
+    class Library(type(opt._lib)):
+        def stochqn_hip_adamw_step(self, *args):
+            opt.update_gradient(None)                       # as the other thread does
+            assert alive() is not None
+            return 0
+
+    opt._lib = Library()
+    with pytest.MonkeyPatch.context() as patch:
+        patch.setattr(adamw, "_stream", lambda index: 10)
+        opt.run_optimizer(0.1)
+    assert alive() is None and opt.gradient is None
 
 
 @pytest.mark.parametrize("which", ["asan", "tsan"])
