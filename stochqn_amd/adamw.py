@@ -299,7 +299,10 @@ class AdamW_free:
         same = ("beta1", "beta2", "eps", "weight_decay", "state_bits", "stochastic", "seed", "decay", "sizes")
         if set(state) != set(mine) or any(state[k] != mine[k] for k in same):
             raise ValueError("the state belongs to an optimizer that was constructed otherwise.")
-        for k in set(mine) - set(same):
+        arrays = set(mine) - set(same)
+        if any(getattr(state[k], "shape", None) != mine[k].shape or state[k].dtype != mine[k].dtype for k in arrays):
+            raise ValueError("the state's arrays have other shapes or types than this optimizer's.")
+        for k in arrays:
             mine[k].copy_(state[k])
 
     def __del__(self):

@@ -175,6 +175,25 @@ def test_the_gradients_live_as_long_as_the_step_that_reads_them():
     assert alive() is None and opt.gradient is None
 
 
+def test_a_state_of_other_shapes_or_types_is_refused_as_a_whole():
+    """Arrays that a copy would spread over the optimizer's, or cast: refused in front of the first copy."""
+    torch = pytest.importorskip("torch")
+
+    def optimizer(fill):
+        sizes = type("Sizes", (), {"sizes": [200]})()
+        return bare_optimizer(torch, params=sizes, m=torch.full((256,), fill), v=torch.full((256,), fill), count=torch.full((2,), int(fill)), beta1=0.9, beta2=0.999,
+                              eps=1e-8, weight_decay=0.0, state_bits=32, stochastic=False, seed=0, decay=None)
+    mine, other = optimizer(1.0), optimizer(2.0)
+    good = other.state_dict()
+    for name in ("m", "v", "count"):
+        for bad in (good[name][:1], good[name].view(2, -1), good[name].to(torch.float16), None, 2.0):
+            with pytest.raises(ValueError):
+                mine.load_state_dict(dict(good, **{name: bad}))
+            assert mine.m.eq(1).all() and mine.v.eq(1).all() and mine.count.eq(1).all(), (name, bad)
+    mine.load_state_dict(good)
+    assert mine.m.eq(2).all() and mine.v.eq(2).all() and mine.count.eq(2).all()
+
+
 @pytest.mark.parametrize("which", ["asan", "tsan"])
 def test_the_host_side_under_sanitizers(which):
     """What tensors.cpp hands to the kernels (every element of every tensor in one tile of one launch) and what it refuses, every HIP call failing
