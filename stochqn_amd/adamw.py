@@ -136,13 +136,17 @@ class TensorList:
         max_norm = math.inf if max_norm is None else float(max_norm)
         if not max_norm > 0 or not math.isfinite(grad_scale):
             raise ValueError("'max_norm' has to be positive and 'grad_scale' finite.")
-        if out is None:
+        mine = out is None
+        if mine:
             out = torch.empty(2, dtype=torch.float32, device=self.device)
-        elif out.dtype != torch.float32 or out.shape != (2,) or out.device != self.device or not out.is_contiguous():
-            raise ValueError("'out' has to be a float32 tensor of two elements on %s." % self.device)
+        elif (not isinstance(out, torch.Tensor) or out.dtype != torch.float32 or out.shape != (2,) or out.device != self.device
+              or out.layout != torch.strided or not out.is_contiguous() or out.is_neg() or out.requires_grad):
+            raise ValueError("'out' has to be a float32 tensor of two elements on %s, of which no gradient is taken." % self.device)
         work = torch.empty(self._work, dtype=torch.float64, device=self.device)      # of this call alone: two streams, or two graphs, share none
         if self._lib.stochqn_hip_tensors_norm(self._handle, grad_scale, max_norm, out.data_ptr(), work.data_ptr(), _stream(self._index)) != 0:
             raise RuntimeError("stochqn_hip_tensors_norm failed (its reason is on stderr).")
+        if not mine and not out.is_inference():
+            torch.autograd.graph.increment_version(out)
         return out
 
     def __del__(self):

@@ -698,6 +698,21 @@ def test_tensors_that_an_address_does_not_tell_are_refused():
     assert opt.count.tolist() == [0, 0]
 
 
+def test_an_output_that_an_address_does_not_tell_is_refused():
+    """A view that negates would read back the opposite of what was written; a tensor that autograd records would not know that it was."""
+    sq = stochqn()
+    grads = sq.TensorList([torch.ones(300, device="cuda")])
+    for bad in (torch._neg_view(torch.zeros(2, device="cuda")), torch.zeros(2, device="cuda", requires_grad=True), [0.0, 0.0]):
+        with pytest.raises(ValueError):
+            grads.norm(out=bad)
+    out = torch.zeros(2, device="cuda")
+    x = torch.ones(2, device="cuda", requires_grad=True)
+    y = (x * out).sum()                                     # saves out for x's gradient
+    grads.norm(out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_a_parameter_that_is_given_other_memory():
     """The old memory stays until the optimizer goes, so nothing is written where others may be by now; the next gradient is refused."""
     sq = stochqn()
