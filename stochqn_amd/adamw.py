@@ -92,8 +92,9 @@ class TensorList:
         self._at = self._addresses(self.tensors)
         self._memory = [t.untyped_storage() for t in self.tensors]       # a tensor that is given other memory (`.data = ...`) lets go of it
         self._lib = _library()
-        self._handle = self._lib.stochqn_hip_tensors_create(n, (C.c_void_p * n)(*self._at), (C.c_size_t * n)(*self.sizes),
-                                                            (C.c_int * n)(*[types[d] for d in self.dtypes]))
+        with torch.cuda.device(self._index):            # where a list of empty tensors alone belongs
+            self._handle = self._lib.stochqn_hip_tensors_create(n, (C.c_void_p * n)(*self._at), (C.c_size_t * n)(*self.sizes),
+                                                                (C.c_int * n)(*[types[d] for d in self.dtypes]))
         if not self._handle:
             raise ValueError("the library refused the tensors (its reason is on stderr).")
         self._work = self._lib.stochqn_hip_tensors_norm_work(self._handle)

@@ -194,6 +194,44 @@ def test_a_state_of_other_shapes_or_types_is_refused_as_a_whole():
     assert mine.m.eq(2).all() and mine.v.eq(2).all() and mine.count.eq(2).all()
 
 
+def test_a_list_of_empty_tensors_belongs_to_their_device(monkeypatch):
+    """The library looks at no address of an empty tensor: a list of nothing else is made while the tensors' device is the current one."""
+    torch = pytest.importorskip("torch")
+    current = [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.was, current[0] = current[0], torch.device(self.index).index if not isinstance(self.index, int) else self.index
+
+        def __exit__(self, *args):
+            current[0] = self.was
+
+    class Library:
+        def stochqn_hip_tensors_create(self, *args):
+            self.on = current[0]
+            return 1
+
+        def stochqn_hip_tensors_norm_work(self, handle):
+            return 1
+
+        def stochqn_hip_tensors_destroy(self, handle):
+            pass
+
+    class Empty:
+        dtype, is_cuda, device, layout = torch.float32, True, torch.device("cuda", 1), torch.strided
+        get_device, numel, data_ptr = lambda self: 1, lambda self: 0, lambda self: 0
+        is_contiguous, is_neg, untyped_storage = lambda self: True, lambda self: False, lambda self: None
+
+    library = Library()
+    monkeypatch.setattr(adamw, "_library", lambda: library)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    adamw.TensorList([Empty(), Empty()])
+    assert library.on == 1 and current[0] == 0
+
+
 @pytest.mark.parametrize("which", ["asan", "tsan"])
 def test_the_host_side_under_sanitizers(which):
     """What tensors.cpp hands to the kernels (every element of every tensor in one tile of one launch) and what it refuses, every HIP call failing
