@@ -378,6 +378,39 @@ static void overlaps_in_a_call()
 	CHECK(norm(work + 8 * doubles, work) == 0 && norm(out, work) == 0 && norm(l.p[0], work) == 0);
 }
 
+// which tile a list's sizes choose, on both sides of every threshold (the stand-in device has 256 units)
+static void tiles_by_size()
+{
+	const auto step = [](const std::vector<size_t>& n, int bits) {
+		Lists l(n);
+		stochqn_hip_adamw_setup s = l.setup(bits);
+		stochqn_hip_adamw* o = stochqn_hip_adamw_create(l.params, &s);
+		g_launches.clear();
+		CHECK(o && stochqn_hip_adamw_step(o, l.grads, 0.1, nullptr, nullptr, nullptr) == 0);
+		stochqn_hip_adamw_destroy(o);
+		return g_launches[0];
+	};
+	const auto norm = [](const std::vector<size_t>& n) {
+		Lists l(n);
+		float* out = (float*) device_block(8);
+		double* work = (double*) device_block(8 * stochqn_hip_tensors_norm_work(l.grads));
+		g_launches.clear();
+		CHECK(stochqn_hip_tensors_norm(l.grads, 1, 1, out, work, nullptr) == 0);
+		return g_launches[0];
+	};
+	const size_t units = 256;
+	for (int bits : {32, 8}) {
+		const size_t tile = bits == 32 ? sqn::kTile32 : sqn::kTile8, few = 8 * units * tile;
+		CHECK(step({few - tile}, bits).tile == sqn::kTileSmall && step({few - tile + 1}, bits).tile == (int) tile && step({few - 2 * tile, 1}, bits).tile == sqn::kTileSmall);
+		CHECK(step({few - 2 * tile, 1, 1}, bits).tile == (int) tile);
+		const size_t most = bits == 32 ? 16 * units : 32 * units;              // workgroups; a list with more tiles goes round
+		CHECK(step({4 * few}, bits).grid == (int) std::min(4 * few / tile, most) && 8 * few / tile > most && step({8 * few}, bits).grid == (int) most);
+	}
+	CHECK(norm({2 * units * sqn::kTileNormMid - sqn::kTileNormMid}).tile == sqn::kTileSmall && norm({2 * units * sqn::kTileNormMid}).tile == sqn::kTileNormMid);
+	CHECK(norm({4 * units * sqn::kTileNorm - sqn::kTileNorm}).tile == sqn::kTileNormMid && norm({4 * units * sqn::kTileNorm}).tile == sqn::kTileNorm);
+	CHECK(norm({9 * units * sqn::kTileNorm}).grid == (int) (8 * units));
+}
+
 // A list that two optimizers read while a third thread rebinds it and a fourth takes its norm: every table is of one binding or the other.
 static void concurrent()
 {
@@ -449,6 +482,7 @@ int main(int argc, char**)
 			covers(n, bits, k);
 		}
 	}
+	tiles_by_size();
 	refusals();
 	overlaps_in_a_call();
 	std::printf("ok\n");

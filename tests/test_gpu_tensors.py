@@ -165,6 +165,137 @@ def test_more_tensors_than_a_launch_takes(bits, count):
     assert abs(float(got[0]) - want) <= 2.0 ** -23 * want
 
 
+class Large:
+    """A list of tensors of given sizes and types, made on the GPU, for `places`."""
+
+    def __init__(self, sizes, ptypes, gtypes, seed=0):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        self.sizes, self.ptypes, self.gtypes = sizes, ptypes, gtypes
+        self.pbuf = [torch.full((n + 2,), 77.0, dtype=t, device="cuda") for n, t in zip(sizes, ptypes)]
+        self.gbuf = [torch.full((n + 2,), 77.0, dtype=t, device="cuda") for n, t in zip(sizes, gtypes)]
+        self.params, self.grads = [b[1:-1] for b in self.pbuf], [b[1:-1] for b in self.gbuf]
+        for k, (p, g) in enumerate(zip(self.params, self.grads)):
+            p.copy_(torch.randn(p.numel(), device="cuda", generator=gen))
+            g.copy_(torch.randn(g.numel(), device="cuda", generator=gen) * 10.0 ** -(k % 5))
+
+    def whole(self):
+        for b in self.pbuf + self.gbuf:
+            assert b[0] == 77 and b[-1] == 77
+
+
+def places(n, tile):
+    """Elements of the first and the last block of 128 of every tile of a tensor, blocks whole."""
+    blocks = -(-n // 128)
+    per = tile // 128
+    first = np.arange(0, blocks, per)
+    pick = np.unique(np.concatenate([first, np.minimum(first + per - 1, blocks - 1)])) if blocks else first
+    return (pick[:, None] * 128 + np.arange(128)).reshape(-1)
+
+
+def check_large_step(model, opt, tile, decay):
+    """One step, its results at `places` held to the reference from the state before: every tile of every tensor is looked at, at both its ends."""
+    b1, b2, eps, wd, t = opt.beta1, opt.beta2, opt.eps, opt.weight_decay, int(opt.count[0]) + 1
+    eight, before = opt.state_bits == 8, []
+    at = [torch.as_tensor(places(n, tile)).cuda() for n in model.sizes]
+
+    def state(x, scale, i, k):
+        e = at[i] + opt.offsets[i]
+        if not eight:
+            return x[e].cpu().numpy()
+        return ref.decode(codes(x.view(torch.uint8)[e]), codes(scale.view(torch.uint8)[e[::128] // 128]), k)
+
+    def values(x, i):
+        got = np.zeros(at[i].numel(), dtype=np.float32)
+        real = (at[i] < model.sizes[i]).cpu().numpy()
+        got[real] = host(x[at[i][at[i] < model.sizes[i]]])
+        return got, real
+
+    for i, n in enumerate(model.sizes):
+        master = opt.master is not None and model.ptypes[i] != F32
+        w = opt.master[opt.offsets[i]:opt.offsets[i] + n] if master else model.params[i]
+        before.append((values(w, i), values(model.grads[i], i)[0], state(opt.m, opt.m_scale, i, "m"), state(opt.v, opt.v_scale, i, "v")))
+    opt.run_optimizer(LR)
+    torch.cuda.synchronize()
+    assert opt.count.tolist() == [t, 0]
+    for i, n in enumerate(model.sizes):
+        (w, real), g, m, v = before[i]
+        if not n:
+            continue
+        w64, m64, v64, w_tol, m_tol, v_tol = ref.step64(w, m, v, g, 1.0, t, LR, b1, b2, eps, wd if decay[i] else 0.0)
+        e = at[i].cpu().numpy().astype(np.uint64) + np.uint64(opt.offsets[i])
+        with np.errstate(over="ignore"):
+            key = ref.finalise(np.uint64((opt.seed ^ (t * ref.STEP_KEY)) & ref.M64))
+            word = ref.finalise(key + (e >> np.uint64(3)) * np.uint64(ref.GOLDEN))
+        lane = (e & np.uint64(7)) * np.uint64(ref.LANE)
+        low, high = (((h + lane) & np.uint64(0xFFFFFFFF)).astype(np.uint32) for h in (word & np.uint64(0xFFFFFFFF), word >> np.uint64(32)))
+        assert (low[:128] == ref.words(int(e[0]), 128, opt.seed, t)[0]).all()
+        if eight:
+            m32, v32 = ref.moments32(m, v, g, 1.0, b1, b2)
+            place = at[i] + opt.offsets[i]
+            for x, scale, x32, k, u in ((opt.m, opt.m_scale, m32, "m", low), (opt.v, opt.v_scale, v32, "v", high)):
+                code, byte = ref.encode(x32, u, k)
+                assert (codes(x.view(torch.uint8)[place]) == code).all() and (codes(scale.view(torch.uint8)[place[::128] // 128]) == byte).all(), (i, k)
+        else:
+            for x, x64, tol in ((state(opt.m, None, i, "m"), m64, m_tol), (state(opt.v, None, i, "v"), v64, v_tol)):
+                assert (np.abs(x - x64) <= tol)[real].all() and not x[~real].any(), i
+        new = values(model.params[i], i)[0][real]
+        w64, w_tol = w64[real], w_tol[real]
+        if model.ptypes[i] == F32:
+            assert (np.abs(new - w64) <= w_tol).all(), i
+        elif opt.master is not None:
+            mast = values(opt.master[opt.offsets[i]:opt.offsets[i] + n], i)[0][real]
+            assert (np.abs(mast - w64) <= w_tol).all() and (torch.as_tensor(mast).to(model.ptypes[i]).float().numpy() == new).all(), i
+        else:
+            lo, hi = (ref.bf16_stochastic(x.astype(np.float32), low[real]) for x in (w64 - 1.01 * w_tol, w64 + 1.01 * w_tol))
+            assert ((lo <= new) & (new <= hi)).all(), i
+    model.whole()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("kw", [dict(master=True), dict(stochastic=True)], ids=["master", "stochastic"])
+@pytest.mark.parametrize("round_trip", [False, True], ids=["a_tile_each", "more_tiles_than_workgroups"])
+def test_large_tiles_over_several_tensors(bits, kw, round_trip):
+    """Lists past the threshold of the large tiles (8 for each compute unit), with as many workgroups as tiles and with more tiles than workgroups, so
+    that a workgroup goes on from one tensor to another of other types, flags and places."""
+    units = torch.cuda.get_device_properties(0).multi_processor_count
+    tile = 4096 if bits == 32 else 8192
+    tiles = units * (10 if not round_trip else 20 if bits == 32 else 38)
+    assert tiles >= 8 * units and (tiles > (16 if bits == 32 else 32) * units) == round_trip
+    part = tiles * tile
+    half = F16 if "master" in kw else BF16
+    sizes = [int(part * 0.31) + 1, 33, 0, int(part * 0.27) + 129, 2047, int(part * 0.24) - 1, 127, int(part * 0.18) + 3]
+    ptypes, gtypes = [F32, BF16, F32, BF16, F32, half, BF16, BF16], [F32, F32, BF16, BF16, BF16, F32, F16, F16]
+    decay = [True, False, True, False, False, True, True, False]
+    assert sum(-(-n // tile) for n in sizes) >= tiles
+    model = Large(sizes, ptypes, gtypes, seed=bits)
+    opt = stochqn().AdamW_free(model.params, state_bits=bits, decay=decay, weight_decay=0.3, seed=5, **kw)
+    opt.update_gradient(model.grads)
+    for _ in range(2):
+        check_large_step(model, opt, tile, decay)
+
+
+@pytest.mark.parametrize("types", [[F32], [BF16], [F16], [F32, BF16, F16]], ids=["f32", "bf16", "f16", "mixed"])
+@pytest.mark.parametrize("tiles", [600, 1100, 2500])
+def test_norm_of_large_lists(types, tiles):
+    """Past each threshold of the norm's tiles (256 compute units: 512 of 8192 elements, 1024 of 16384), and with more tiles than workgroups (2048)."""
+    assert torch.cuda.get_device_properties(0).multi_processor_count == 256
+    part = tiles * (8192 if tiles < 1024 else 16384)
+    sizes = [int(part * 0.4) + 1, 5, int(part * 0.35) - 1, 0, 2049, int(part * 0.25) + 7]
+    kinds = [types[k % len(types)] for k in range(len(sizes))]
+    model = Large(sizes, kinds, kinds, seed=tiles)
+    grads = stochqn().TensorList(model.grads)
+    for k in range(2):
+        want = math.sqrt(sum(float(g.double().square().sum()) for g in model.grads))
+        out = grads.norm(max_norm=1.0)
+        # f64 sums in two orders, in each of which an element goes through fewer than 1e4 additions (1e4 * 2^-53 is nothing beside a hundredth of 2^-24),
+        # then one rounding to f32 each
+        assert abs(float(out[0]) - want) <= 1.01 * 2.0 ** -24 * want and abs(float(out[1]) - 1 / want) <= 1.01 * 2.0 ** -24 / want
+        assert torch.equal(grads.norm(max_norm=1.0), out)
+        model.grads[0][-1] = 1e4                            # the last element of a tensor counts
+        model.grads[-1][-1] = 3e4
+    model.whole()
+
+
 def test_only_empty_tensors():
     model = Model([0, 0], F32, F32)
     opt = stochqn().AdamW_free(model.params)
@@ -659,6 +790,39 @@ def test_the_first_steps_with_adamw_the_rest_with_sqn():
             qn.update_gradient(d * on)
         r = qn.run_optimizer(x, 0.1)
     assert torch.isfinite(x).all() and float((d * x * x).sum()) < loss[0]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_on_a_problem_then_sqn(bits):
+    """A noisy quadratic: clipped steps whose gradients follow from the weights, each held to the reference, then SQN on the vector that they leave."""
+    sq = stochqn()
+    rng = np.random.default_rng(1)
+    sizes, n = [640, 256, 104], 1000
+    d = torch.as_tensor(0.5 + rng.random(n)).float().cuda()
+    model = Model(sizes, F32, F32, gap=0, seed=4)
+    cuts = list(zip(torch.split(d, sizes), model.params, model.grads))
+    opt = sq.AdamW_free(model.params, state_bits=bits, seed=8)
+    grads = sq.TensorList(model.grads)
+    opt.update_gradient(grads)
+    for _ in range(60):
+        for part, p, g in cuts:
+            g.copy_(part * p + 0.1 * torch.as_tensor(rng.standard_normal(p.numel())).float().cuda())
+        clip = grads.norm(max_norm=1.0)
+        want = math.sqrt(sum(float(g.double().square().sum()) for g in model.grads))
+        assert abs(float(clip[1]) - min(1.0, 1.0 / want)) <= 1.01 * 2.0 ** -24
+        check_step(model, opt, scale=float(clip[1]), grad_scale=clip[1:])
+    x = torch.cat(model.params).double()
+    was = x.clone()
+    qn = sq.SQN_free(mem_size=5, bfgs_upd_freq=3, space="device")
+    r = qn.run_optimizer(x, 0.1)
+    for _ in range(60):
+        on = r["requested_on"]
+        if r["task"] == "calc_hess_vec":
+            qn.update_hess_vec(d.double() * on[1])
+        else:
+            qn.update_gradient(d.double() * on)
+        r = qn.run_optimizer(x, 0.1)
+    assert torch.isfinite(x).all() and not x.eq(was).any()
 
 
 def test_memory_that_a_step_or_a_norm_both_reads_and_writes_is_refused():
