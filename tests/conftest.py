@@ -74,10 +74,11 @@ def pytest_configure(config):
 
 
 def pytest_collection_modifyitems(items):
-    """The tests that count page-locked ranges come last: some machines refuse to page-lock memory that exists already (hipHostRegister), and a run
-    that ends at its first failure has then seen everything else.  Nothing is left out, and the order within a file stays."""
+    """The tests that need what not every machine has come last: those that count page-locked ranges (some machines refuse to page-lock memory that
+    exists already, hipHostRegister) and those that compile the reference's own sources (its folder may be there and be empty).  A run that ends at its
+    first failure has then seen everything else.  Nothing is left out, and the order within a file stays."""
     last = ("test_gpu_devices.py", "test_gpu_host_path.py")
-    items.sort(key=lambda item: item.path.name in last)
+    items.sort(key=lambda item: item.path.name in last or item.name.startswith("test_reference_"))
 
 
 @pytest.fixture(scope="session")
