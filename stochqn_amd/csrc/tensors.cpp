@@ -79,9 +79,16 @@ void check_aligned(const void* p, size_t to, const char* what)
 
 uint64_t tiles_of(size_t n, int tile) { return (n + tile - 1) / tile; }
 
-// Large tiles keep more loads of a lane in flight; a list with fewer than `few` of them for each compute unit is cut into smaller ones, so that
-// every unit has work.  Measured at 7.7e6 elements: the step with 8-bit moments 21.7 us small, 24.1 large (3.7 large tiles a unit), with 32-bit
-// moments 40.3 and 44.8 (7.4 a unit); the norm 12.6 us with tiles of 2048, 9.3 with 8192 (3.7 a unit), 10.3 with 16384 (1.8).
+// Large tiles keep more loads of a lane in flight; a list with fewer than `few` of them for each compute unit is cut into smaller ones, whose
+// kernels need fewer registers (80 against 122, 92 against 156 with 8-bit moments: more waves a unit).  Where the two meet, in us with small and with large tiles at that many large
+// tiles a unit (one vector; lists of layers are alike):
+//   8-bit moments   f32:         8: 51.1 57.4   16: 103 107   24: 157 156   32: 211 204   48: 323 307   128: 907 816
+//                   bf16 alone:  8: 35.7 39.1   16: 63.3 68.0   32: 120 128   48: 190 190   64: 250 250   128: 592 487      -> 32
+//   32-bit moments  f32:         8: 42.8 44.9   16: 83.4 85.1   32: 162 165   48: 243 245   64: 318 309   96: 478 455      -> 64
+//                   bf16 alone:  8: 34.0 36.0   32: 125 130   64: 245 251   96: 374 371   128: 508 493
+//   the norm (small, 8192, 16384 elements; at that many tiles of 16384 a unit)
+//                   bf16:  1: 9.1 9.4 8.9   3: 9.5 9.5 9.2   4: 10.6 10.1 10.8   6: 13.2 12.4 13.1   8: 15.7 15.3 15.5   16: 25.5 25.1 24.8   32: 44.7 45.0 43.4
+//                   f32:   1: 8.8 9.6 9.5   2: 10.8 10.5 10.1   4: 16.3 16.0 15.8   8: 27.1 26.4 26.3   16: 49.2 47.5 47.4   32: 93.6 89.9 89.4      -> 2 of 8192, 4 of 16384
 LaunchShape shape_of(const std::vector<Item>& items, int units, int per_unit, std::initializer_list<std::pair<int, int>> tile_and_few)
 {
 	for (const auto& [tile, few] : tile_and_few) {
@@ -331,7 +338,7 @@ stochqn_hip_adamw* stochqn_hip_adamw_create(stochqn_hip_tensors* params, const s
 		std::lock_guard<std::mutex> lk(params->mu);
 		o->items = params->items;
 		o->device = params->device;
-		o->shape = s.state_bits == 8 ? shape_of(o->items, params->units, kPerUnit8, {{kTile8, 8}}) : shape_of(o->items, params->units, kPerUnit32, {{kTile32, 8}});
+		o->shape = s.state_bits == 8 ? shape_of(o->items, params->units, kPerUnit8, {{kTile8, 32}}) : shape_of(o->items, params->units, kPerUnit32, {{kTile32, 64}});
 		o->s = s;
 		size_t blocks = 0;
 		for (size_t i = 0; i < o->items.size(); i++) {

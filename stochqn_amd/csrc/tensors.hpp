@@ -10,15 +10,17 @@ namespace sqn {
 
 constexpr int kStateBlock = 128;     // elements that share the scale of an 8-bit moment; every tensor's state starts at a multiple of it
 // Elements a workgroup of 256 threads takes at a time, their loads issued together.  Measured: the step with 32-bit moments at 1e8 f32
-// elements 533 us with tiles of 2048, 474 with 4096, 531 with 8192 (two waves a SIMD); with 8-bit moments at 1.28e9 bf16 elements 2.79, 2.60, 2.40 ms
-// (3.04 with 16384); the norm of those 396, 392, 395 us and 379 with 16384, of 7.7e6 elements 12.6, 9.6, 9.3 and 10.3 us.
+// elements 482 us with tiles of 2048, 473 with 4096, 535 with 8192, at 1.28e9 bf16 + f32 elements 6.99, 6.50 and 7.72 ms; with 8-bit moments at 1.28e9 bf16
+// elements 2.58 ms with 4096, 2.40 with 8192 (16384 spill: 14.9); the norm of those 396, 392, 395 us and 379 with 16384, of 7.7e6 elements 12.6, 9.6, 9.3
+// and 10.3 us.
 constexpr int kTileSmall = 2048;     // lists that would not fill the card otherwise (tensors.cpp: shape_of)
 constexpr int kTile32 = 4096;        // moments in 32 bits
 constexpr int kTile8 = 8192;         // in 8 bits
 constexpr int kTileNormMid = 8192;   // the norm
 constexpr int kTileNorm = 16384;
 constexpr int kEntries = 112;        // tensors per launch: the table travels in the kernel's arguments (32 B each, 4 KB in all)
-constexpr int kFewEntries = 12;      // ... of a short list, whose launch then costs less
+constexpr int kFewEntries = 12;      // ... of a short list: 3.6 KB less for the host to hand over, 0.1 - 0.3 us of a call (12 tensors: 5.7 against 5.8 us, their norm 8.6
+                                     // against 8.8); the GPU's time is the same (5.16 and 5.15 us a step), with 40 entries too
 
 enum TensorType { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
 inline size_t type_size(int t) { return t == T_F32 ? 4 : 2; }

@@ -400,11 +400,12 @@ static void tiles_by_size()
 	};
 	const size_t units = 256;
 	for (int bits : {32, 8}) {
-		const size_t tile = bits == 32 ? sqn::kTile32 : sqn::kTile8, few = 8 * units * tile;
+		const size_t tile = bits == 32 ? sqn::kTile32 : sqn::kTile8, few = (bits == 32 ? 64 : 32) * units * tile;
 		CHECK(step({few - tile}, bits).tile == sqn::kTileSmall && step({few - tile + 1}, bits).tile == (int) tile && step({few - 2 * tile, 1}, bits).tile == sqn::kTileSmall);
 		CHECK(step({few - 2 * tile, 1, 1}, bits).tile == (int) tile);
 		const size_t most = bits == 32 ? 16 * units : 32 * units;              // workgroups; a list with more tiles goes round
-		CHECK(step({4 * few}, bits).grid == (int) std::min(4 * few / tile, most) && 8 * few / tile > most && step({8 * few}, bits).grid == (int) most);
+		CHECK(step({few}, bits).grid == (int) most && step({2 * few}, bits).grid == (int) most && step({most * sqn::kTileSmall - 1, 1}, bits).grid == (int) most);
+		CHECK(step({most * sqn::kTileSmall - sqn::kTileSmall}, bits).grid == (int) most - 1);
 	}
 	CHECK(norm({2 * units * sqn::kTileNormMid - sqn::kTileNormMid}).tile == sqn::kTileSmall && norm({2 * units * sqn::kTileNormMid}).tile == sqn::kTileNormMid);
 	CHECK(norm({4 * units * sqn::kTileNorm - sqn::kTileNorm}).tile == sqn::kTileNormMid && norm({4 * units * sqn::kTileNorm}).tile == sqn::kTileNorm);

@@ -253,20 +253,21 @@ def check_large_step(model, opt, tile, decay):
 
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("kw", [dict(master=True), dict(stochastic=True)], ids=["master", "stochastic"])
-@pytest.mark.parametrize("round_trip", [False, True], ids=["a_tile_each", "more_tiles_than_workgroups"])
-def test_large_tiles_over_several_tensors(bits, kw, round_trip):
-    """Lists past the threshold of the large tiles (8 for each compute unit), with as many workgroups as tiles and with more tiles than workgroups, so
-    that a workgroup goes on from one tensor to another of other types, flags and places."""
+@pytest.mark.parametrize("tile", [2048, "large"])
+def test_large_lists_of_several_tensors(bits, kw, tile):
+    """Lists on both sides of the threshold of the large tiles (64 and 32 of them for each compute unit), with more tiles than workgroups, so that a
+    workgroup goes on from one tensor to another of other types, flags and places."""
     units = torch.cuda.get_device_properties(0).multi_processor_count
-    tile = 4096 if bits == 32 else 8192
-    tiles = units * (10 if not round_trip else 20 if bits == 32 else 38)
-    assert tiles >= 8 * units and (tiles > (16 if bits == 32 else 32) * units) == round_trip
+    large, few, workgroups = (4096, 64, 16 * units) if bits == 32 else (8192, 32, 32 * units)
+    tiles = workgroups * 5 // 4 if tile == 2048 else units * few * 9 // 8
+    tile = large if tile == "large" else tile
+    assert tiles > workgroups and (tiles * tile // large >= few * units) == (tile == large)
     part = tiles * tile
     half = F16 if "master" in kw else BF16
     sizes = [int(part * 0.31) + 1, 33, 0, int(part * 0.27) + 129, 2047, int(part * 0.24) - 1, 127, int(part * 0.18) + 3]
     ptypes, gtypes = [F32, BF16, F32, BF16, F32, half, BF16, BF16], [F32, F32, BF16, BF16, BF16, F32, F16, F16]
     decay = [True, False, True, False, False, True, True, False]
-    assert sum(-(-n // tile) for n in sizes) >= tiles
+    assert sum(-(-n // tile) for n in sizes) >= tiles and (sum(-(-n // large) for n in sizes) >= few * units) == (tile == large)
     model = Large(sizes, ptypes, gtypes, seed=bits)
     opt = stochqn().AdamW_free(model.params, state_bits=bits, decay=decay, weight_decay=0.3, seed=5, **kw)
     opt.update_gradient(model.grads)
