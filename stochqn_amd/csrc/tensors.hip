@@ -431,7 +431,7 @@ template <int TILE> struct Tile8 {
 
 // Every wave reads the step counter and forms the step's numbers itself, while its first tile is on the way.  One thread of a workgroup arrives
 // for its four waves, behind a barrier: only there have all of them read the counter (their stores wait for what they made of it).  The last
-// workgroup to arrive counts the step.  (A kernel in front that did both cost 3.5 us a step; arrivals at one counter cost 6 us at 1000 workgroups.)  One launch of one workgroup takes 2.8 - 3.2 us.
+// workgroup to arrive counts the step.  (A kernel in front that did both cost 3.5 us a step; arrivals at one counter cost 6 us at 1000 workgroups.)  One launch of one workgroup takes 2.8 - 3.4 us.
 template <template <int> class Tile, int TILE, int N> __global__ __launch_bounds__(kThreads) void k_adamw(const Table<AdamwArgs, N> table)
 {
 	const AdamwArgs& a = table.a;
