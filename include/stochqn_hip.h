@@ -301,7 +301,7 @@ int stochqn_hip_tensors_norm(stochqn_hip_tensors *tensors, double grad_scale, do
  *                     of two (e8m0) that 128 elements share.  A moment is code * scale, rounded stochastically -- to one of its two
  *                     neighbours, each as often as the mean asks for; rounding to nearest would never move v again, which changes by
  *                     1 - beta2 a step -- by words that depend on (seed, t, place) alone.  v > 0 is held above zero.  A block in which a
- *                     moment is not finite reads as NaN from then on.
+ *                     moment is not finite, or is rounded past f32, reads as NaN from then on.
  *   master            f32[state] or NULL: weights that the step is taken on where a parameter has 16 bits (the parameter is written, rounded,
  *                     and not read); unused for f32 parameters
  *   stochastic        without master: bf16 parameters are rounded stochastically as well (no f16 parameters then)
