@@ -13,7 +13,7 @@ constexpr int kStateBlock = 128;     // elements that share the scale of an 8-bi
 // elements 482 us with tiles of 2048, 473 with 4096, 535 with 8192, at 1.28e9 bf16 + f32 elements 6.99, 6.50 and 7.72 ms; with 8-bit moments at 1.28e9 bf16
 // elements 2.58 ms with 4096, 2.40 with 8192 (16384 spill: 14.9); the norm of those 396, 392, 395 us and 379 with 16384, of 7.7e6 elements 12.6, 9.6, 9.3
 // and 10.3 us.
-constexpr int kTileSmall = 2048;     // lists that would not fill the card otherwise (tensors.cpp: shape_of)
+constexpr int kTileSmall = 2048;     // short lists: both sides measured at the rule (tensors.cpp: shape_of)
 constexpr int kTile32 = 4096;        // moments in 32 bits
 constexpr int kTile8 = 8192;         // in 8 bits
 constexpr int kTileNormMid = 8192;   // the norm
